@@ -16,7 +16,8 @@
  *   *_host  : caller passes host buffers (what the per-call C++ API hands over); the library packs,
  *             uploads, launches, downloads.  Synchronous, thread-safe (internal lock).
  *   *_dev   : caller passes device-resident SoA buffers (HBM) and a stream; nothing is copied, the call
- *             only enqueues kernels.  This is the throughput path fed at the BamProcessor batch boundary
+ *             only enqueues kernels (and, where a per-read constant goes through the C library's log / exp / logf, a
+ *             host function of the stream: see "per-read constants" below).  This is the throughput path fed at the BamProcessor batch boundary
  *             (src/common/nanopolish_bam_processor.cpp:90-119).
  */
 #ifndef NP_HMM_H
@@ -85,7 +86,7 @@ const char* np_ctx_info(const np_ctx* ctx);
  * (1: np_hmm_score_host sends a small batch as one pinned blob; 0: the general path -- the tests compare the two).
  * Environment, read at np_create (each the option of the same name): NP_ALIGN_BLOCKS_PER_CU, NP_HMM_BLOCKS_PER_CU, NP_ALIGN_LPT, NP_ED_WARMUP, NP_ED_RATIO_EXACT,
  * NP_EA_WAVES_PER_CU, NP_RECAL_SHAPE; NP_EA_WALK_PRIO=1 runs the chain kernel's back-track at wave priority 3 (measured slower,
- * profiles/r05_soak.md); NP_LSE_CLAMP, NP_HOST_CONSTANTS, NP_VERBOSE as described at np_ctx_info / in INTEGRATION.md. */
+ * profiles/r05_soak.md); NP_LSE_CLAMP, NP_HOST_CONSTANTS (0 is refused), NP_VERBOSE as described at np_ctx_info / in INTEGRATION.md. */
 int np_set_option(np_ctx* ctx, const char* name, int64_t value);
 /* Read-only facts about the context (-1: unknown name): "align_blocks" / "align_scratch_bytes" (persistent grid and per-wave scratch
  * of the most recent event-align launch: the grid shrinks under a 48 GB scratch budget when a batch holds ultra-long reads),
@@ -205,7 +206,12 @@ int np_event_align_host(np_ctx* ctx, int n_jobs, const np_align_job* jobs,
  * *_host call, which uses the context's own stream), the library makes the new stream wait for everything enqueued on the
  * old one (an event wait on the device, nothing blocks the host).  For concurrent pipelines create one context per stream.
  * Scratch grows on demand: the first call at a larger batch size reallocates (a device-wide synchronisation); steady-state
- * calls do not. */
+ * calls do not.
+ * Per-read constants: the aligner's lp_*, the HMM transitions, set4's log(var) and profile_hmm_score_set's log(n) are the bits of the
+ * C library that the reference runs on, so the PROCESS's own log / exp / logf form them.  np_mom_fill_dev, np_resolve_jobs_dev,
+ * np_calibrate_resolve_dev and np_hmm_score_set_combine_dev enqueue a kernel that writes what they depend on into pinned host
+ * memory, a host function (hipLaunchHostFunc) and a kernel that reads them back: in stream order, the caller does not wait.  These four
+ * cannot be captured into a graph (NP_ERR_UNSUPPORTED). */
 
 /* Per-read record (device).  Filled by np_fill_read_host() on the host, then uploaded by the caller. */
 typedef struct np_read_dev {
@@ -338,15 +344,13 @@ int np_calibrate_resolve_dev(np_ctx* ctx, void* stream, int n_reads, np_read_dev
                              int32_t* map_start, int32_t* map_stop, double* events_per_base, int32_t* calibrated,
                              int64_t n_jobs, np_hmm_job_dev* jobs, const int32_t* kpos);
 
-/* The event aligner's per-read constants {lp_skip, lp_stay, lp_step, lp_trim} (src/nanopolish_raw_loader.cpp:99-108) computed
- * with the library's restatement of glibc's log/exp (csrc/np_log.h) -- what np_mom_fill_dev computes on the device -- and
- * the restated functions themselves (out_log[i] = log(x[i]), out_exp[i] = exp(-x[i])); host-only, for verification. */
+/* The event aligner's per-read constants {lp_skip, lp_stay, lp_step, lp_trim} (src/nanopolish_raw_loader.cpp:99-108) as np_mom_fill_dev's
+ * host function forms them, and the functions that they go through, the process's own (out_log[i] = log(x[i]), out_exp[i] = exp(-x[i]),
+ * NaN where |x[i]| >= 512: no log-probability); host-only, for verification. */
 void np_aligner_constants(uint32_t n_events, uint32_t n_kmers, double out[4]);
 void np_restated_log_exp(const double* x, size_t n, double* out_log, double* out_exp);
-/* Host-only: the restated log / exp / logf against THIS host's libm on n pseudo-random arguments of the ranges the path uses;
- * *n_mismatch == 0 means the constants the device computes are bit-identical to what the reference computes on this host
- * (glibc 2.35 x86-64 with FMA does; another libm may not -- the restatement then still matches the build this repository
- * was verified against, tests/test_host_logic.py reports the difference). */
+/* Host-only: how many of the constants' log / exp / logf values differ from this process's functions: 0, since those functions form
+ * them (kept for callers of the ABI's earlier form, which formed them on the device). */
 int  np_selftest_libm(uint64_t n, uint64_t seed, uint64_t* n_mismatch);
 
 /* ---- f3: work-item generation on the device ------------------------------------------------ */
@@ -513,7 +517,7 @@ int np_detect_events_host(np_ctx* ctx, int n_reads, const float* const* raw, con
 
 /* estimate_scalings_using_mom (src/nanopolish_raw_loader.cpp:30-75) + the event aligner's per-read constants (:99-108) on the
  * device: completes reads[r] (event_off, rank_off, n_kmers already set by the caller) with n_events, shift/scale (var = 1)
- * and lp_skip/lp_stay/lp_step/lp_trim, computed with glibc's log/exp restated (csrc/np_log.h).  reads_b (nullable): a second
+ * and lp_skip/lp_stay/lp_step/lp_trim (by the process's log / exp, see "per-read constants" above).  reads_b (nullable): a second
  * record array (the one kernel B reads) that receives n_events. */
 int np_mom_fill_dev(np_ctx* ctx, void* stream, int n_reads, np_read_dev* reads, np_read_dev* reads_b, const float* event_mean,
                     const int32_t* n_events, const uint16_t* kmer_rank, int model);

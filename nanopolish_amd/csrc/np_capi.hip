@@ -10,8 +10,11 @@
 #include <string>
 #include <vector>
 #include <algorithm>
+#include <atomic>
+#include <memory>
+#include <thread>
 #include "np_kernels.h"
-#include "np_logf.h"
+#include "np_constants.h"
 
 #define NP_VERSION_STR "nanopolish_amd 0.1 (gfx950)"
 #define NP_FLANK_LEN NP_MAX_WINDOW_EVENTS
@@ -36,6 +39,23 @@ struct dev_buf {
     }
     void release() { if (p) (void)hipFree(p); p = nullptr; cap = 0; }
     template <class T> T* as() const { return (T*)p; }
+};
+
+// pinned host memory that kernels and a host function share (host_fix)
+struct host_buf {
+    char* p = nullptr;
+    size_t cap = 0;
+    hipError_t reserve(size_t bytes)
+    {
+        if (bytes <= cap) return hipSuccess;
+        // an earlier call's kernels or host function may still be using the old block
+        if (p) { hipError_t e = hipDeviceSynchronize(); if (e != hipSuccess) return e; e = hipHostFree(p); p = nullptr; cap = 0; if (e != hipSuccess) return e; }
+        const size_t want = bytes + bytes / 4 + 256;
+        hipError_t e = hipHostMalloc((void**)&p, want, hipHostMallocMapped | hipHostMallocCoherent);
+        if (e == hipSuccess) cap = want; else p = nullptr;
+        return e;
+    }
+    void release() { if (p) (void)hipHostFree(p); p = nullptr; cap = 0; }
 };
 
 struct model_t {
@@ -89,8 +109,9 @@ struct np_ctx {
     std::string err;
     int align_blocks_per_cu = 8, hmm_blocks_per_cu = 2;
     int hmm_prio = 0;                 // wave priority of the forward kernels
-    bool host_constants = false;      // the per-read constants that go through libm are computed on the HOST with the process's own log / exp / logf (np_create)
-    double* d_log_n = nullptr;        // host_constants: log(1 .. 64) for profile_hmm_score_set's penalty
+    host_buf hc_align, hc_resolve, hc_sets;      // host_fix: one block per kind of call, so that stages of two batches on two streams do not share one
+    dev_buf hc_var;                   // np_calibrate_resolve_dev: the recalibration's var per read (negative: the read was not rescaled)
+    double lp_skip = 0.0, lp_trim = 0.0; np_trans trans{};      // the aligner constants and transitions that do not depend on the read
     np_slots lay = {nullptr, nullptr, 0}; int64_t lay_total = 0;   // np_set_job_layout: the slot layout of the work-item arrays of the calls that follow
     int recal_shape = 3;              // the recalibration kernel's workgroup shape (3: round 6's half-wave form, the default; 0 ... 2: rounds 5's shapes, same results)
     int align_lpt = 1;                // issue the event aligner's reads longest first
@@ -174,59 +195,107 @@ int persistent_blocks(np_ctx* c, int64_t work_items, int per_block, int blocks_p
     return (int)std::min(need, maxb);
 }
 
-// ---- host-constants mode ----------------------------------------------------------------------------------
-// The device forms the aligner constants (raw_loader.cpp:99-108), set4's log(var) (squiggle_read.cpp:38-65), the HMM transitions
-// (r9.inl:17-76) and profile_hmm_score_set's log(n) with a restatement of THIS image's glibc 2.35 (np_log.h, np_logf.h).  A reference
-// built against another libm computes those constants with ITS log / exp / logf, possibly one ulp away, and "event indices bit-exact"
-// would be gone with no way back short of a rebuild.  np_create therefore compares the restatement with the process's libm
-// (np_selftest_libm); on a mismatch -- or with NP_HOST_CONSTANTS=1 -- the fused pass stops at the three places a constant is formed,
-// reads back what it depends on (two integers, one double per read), computes it on the host with the process's own libm exactly as
-// the reference's expressions do, and uploads it: a few stream synchronisations per batch instead of none, bit-identical to the
-// process's libm whatever it is (tests/test_gpu_libm.py runs the chain under an LD_PRELOADed libm whose log / exp / logf are skewed).
-void transitions_libm(double events_per_base, double indel_bias, float out[10])
+// ---- the constants that go through the C library's log / exp / logf ---------------------------------------------------------------
+// The aligner's lp_stay / lp_step (raw_loader.cpp:99-108), set4's log(var) (squiggle_read.cpp:38-65), the HMM transitions
+// (r9.inl:17-76) and profile_hmm_score_set's log(n) depend on numbers that only exist on the device, and the reference's bits for them
+// are its C library's (np_constants.h).  So they are formed by the process's own functions, in stream order and without making the
+// caller wait:
+//     a kernel writes what they depend on (two integers, one or two doubles per read) into pinned host memory
+//     -> hipLaunchHostFunc: a host function of the stream forms the constants there
+//     -> a kernel copies them into the read records.
+// The call still only enqueues.  (The bytes cross the bus as the kernels' own stores and loads: a copy would queue behind another
+// stream's bulk upload in the copy engine.)  The host function makes no HIP call and throws nothing.
+enum { FIX_ALIGNER, FIX_RESOLVE, FIX_SETS };
+struct host_fix {
+    int what;
+    int64_t n;
+    double indel_bias;
+    const uint2* lengths; double2* lp;                                      // FIX_ALIGNER: (n_events, n_kmers) -> (lp_stay, lp_step)
+    const double* epb; const double* var; float2* mm; double* log_var;      // FIX_RESOLVE: events_per_base -> (lp_mm_self, lp_mm_next), var -> log(var)
+    const int64_t* sizes; double* log_n;                                    // FIX_SETS: n -> log(n)
+
+    void range(int64_t lo, int64_t hi) const noexcept
+    {
+        if (what == FIX_ALIGNER) {
+            const double exp_lp_skip = exp(log(NP_ALIGN_EPSILON));
+            for (int64_t i = lo; i < hi; ++i) { double2 v; np_aligner_lp(lengths[i].x, lengths[i].y, exp_lp_skip, &v.x, &v.y); lp[i] = v; }
+        } else if (what == FIX_RESOLVE) {
+            for (int64_t i = lo; i < hi; ++i) {
+                float p[10];
+                np_transition_probs(epb[i], indel_bias, p);
+                mm[i] = float2{logf(p[0]), logf(p[3])};
+                if (var && !(var[i] < 0.0)) log_var[i] = log(var[i]);       // (negative: not rescaled, its log_var stays)
+            }
+        } else {
+            for (int64_t i = lo; i < hi; ++i) log_n[i] = sizes[i] > 0 ? log((double)(uint64_t)sizes[i]) : 0.0;
+        }
+    }
+    // ~10-30 ns an item: a large batch is shared with a few threads (one more only if the system gives it)
+    void run() const noexcept
+    {
+        const int64_t chunk = 4096;
+        std::atomic<int64_t> next(0);
+        auto work = [&]() { for (int64_t lo; (lo = next.fetch_add(chunk)) < n;) range(lo, std::min(n, lo + chunk)); };
+        std::thread helper[7];
+        int nh = 0;
+        try { for (; nh < 7 && (nh + 2) * 2 * chunk <= n; ++nh) helper[nh] = std::thread(work); } catch (...) {}
+        work();
+        for (int i = 0; i < nh; ++i) helper[i].join();
+    }
+};
+void host_fix_entry(void* p) { std::unique_ptr<host_fix> f((host_fix*)p); f->run(); }
+
+hipError_t enqueue_host_fix(hipStream_t s, const host_fix& f)
 {
-    double read_events_per_base = events_per_base;
-    read_events_per_base *= indel_bias;
-    read_events_per_base = read_events_per_base > 1.25 ? read_events_per_base : 1.25;
-    const float p_stay = (float)(1 - (1 / read_events_per_base));
-    const float p_skip = 0.0025f, p_bad = 0.001f, p_bad_self = p_bad, p_skip_self = 0.3f;
-    const float p_mk = p_skip, p_mb = p_bad, p_mm_self = p_stay;
-    const float p_mm_next = 1.0f - p_mm_self - p_mk - p_mb;
-    const float p_bb = p_bad_self;
-    const float p_bk = (1.0f - p_bb) / 3;
-    const float p_bm_next = p_bk, p_bm_self = p_bk;
-    const float p_kk = p_skip_self;
-    const float p_km = 1.0f - p_kk;
-    const float p[10] = {p_mm_self, p_mb, p_mk, p_mm_next, p_bb, p_bk, p_bm_next, p_bm_self, p_kk, p_km};
-    for (int i = 0; i < 10; ++i) out[i] = logf(p[i]);                       // the float overload of log, as r9.inl:61-72
+    std::unique_ptr<host_fix> own(new (std::nothrow) host_fix(f));
+    if (!own) return hipErrorOutOfMemory;
+    const hipError_t e = hipLaunchHostFunc(s, host_fix_entry, own.get());
+    if (e == hipSuccess) (void)own.release();                               // the host function owns it from here on
+    return e;
 }
 
-// what: 1 = the aligner constants from (n_events, n_kmers); 2 = the transitions from events_per_base; 4 = log_var from var
-int host_constants_fix(np_ctx* c, hipStream_t s, int n_reads, np_read_dev* reads, const double* events_per_base, int what)
+// lp_skip / lp_stay / lp_step / lp_trim of every read from its n_events and n_kmers
+int fix_aligner(np_ctx* c, hipStream_t s, int n_reads, np_read_dev* reads)
 {
     if (n_reads <= 0) return NP_OK;
-    std::vector<np_read_dev> h((size_t)n_reads);
-    std::vector<double> epb;
-    NP_HIP(c, hipMemcpyAsync(h.data(), reads, h.size() * sizeof(np_read_dev), hipMemcpyDeviceToHost, s));
-    if (what & 2) { epb.resize((size_t)n_reads); NP_HIP(c, hipMemcpyAsync(epb.data(), events_per_base, epb.size() * sizeof(double), hipMemcpyDeviceToHost, s)); }
-    NP_HIP(c, hipStreamSynchronize(s));
-    for (int r = 0; r < n_reads; ++r) {
-        np_read_dev& q = h[(size_t)r];
-        if (what & 1) {                                                     // raw_loader.cpp:99-108
-            const double events_per_kmer = (double)q.n_events / (double)q.n_kmers;
-            const double p_stay = 1 - (1 / (events_per_kmer + 1));
-            const double epsilon = 1e-10;
-            q.lp_skip = log(epsilon);
-            q.lp_stay = log(p_stay);
-            q.lp_step = log(1.0 - exp(q.lp_skip) - exp(q.lp_stay));
-            q.lp_trim = log(0.01);
-        }
-        if (what & 2) transitions_libm(epb[(size_t)r], c->params.hmm_indel_bias_factor, q.trans);
-        if (what & 4) q.log_var = log(q.var);                               // set4 / set6, squiggle_read.cpp:38-65
-    }
-    NP_HIP(c, hipMemcpyAsync(reads, h.data(), h.size() * sizeof(np_read_dev), hipMemcpyHostToDevice, s));
-    NP_HIP(c, hipStreamSynchronize(s));                                     // (h is this call's)
+    const size_t n = (size_t)n_reads;
+    NP_HIP(c, c->hc_align.reserve(n * (sizeof(double2) + sizeof(uint2))));
+    host_fix f{};
+    f.what = FIX_ALIGNER; f.n = n_reads;
+    f.lp = (double2*)c->hc_align.p;
+    uint2* const lengths = (uint2*)(f.lp + n);
+    f.lengths = lengths;
+    NP_HIP(c, np_launch_gather_lengths(n_reads, reads, lengths, s));
+    NP_HIP(c, enqueue_host_fix(s, f));
+    NP_HIP(c, np_launch_apply_aligner(n_reads, reads, f.lp, c->lp_skip, c->lp_trim, s));
     return NP_OK;
+}
+// the transitions of every read from events_per_base and, after a calibration (new_var), log_var of the reads that it rescaled
+int fix_resolve(np_ctx* c, hipStream_t s, int n_reads, np_read_dev* reads, const double* events_per_base, const double* new_var)
+{
+    if (n_reads <= 0) return NP_OK;
+    const size_t n = (size_t)n_reads;
+    NP_HIP(c, c->hc_resolve.reserve(n * (3 * sizeof(double) + sizeof(float2))));
+    host_fix f{};
+    f.what = FIX_RESOLVE; f.n = n_reads; f.indel_bias = c->params.hmm_indel_bias_factor;
+    double* const epb = (double*)c->hc_resolve.p;
+    double* const var = epb + n;
+    f.epb = epb; f.var = new_var ? var : nullptr;
+    f.log_var = var + n; f.mm = (float2*)(f.log_var + n);
+    NP_HIP(c, np_launch_gather_resolve(n_reads, events_per_base, new_var, epb, var, s));
+    NP_HIP(c, enqueue_host_fix(s, f));
+    NP_HIP(c, np_launch_apply_resolve(n_reads, reads, f.mm, f.log_var, new_var, c->trans, s));
+    return NP_OK;
+}
+
+// a host function of the stream cannot be replayed from a captured graph here (its argument block lives for one run)
+int refuse_capture(np_ctx* c, void* stream, const char* what)
+{
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    NP_HIP(c, hipStreamIsCapturing(pick_stream(c, stream), &st));
+    if (st == hipStreamCaptureStatusNone) return NP_OK;
+    c->err = std::string(what) + ": cannot be captured into a graph (a host function forms its constants)";
+    return NP_ERR_UNSUPPORTED;
 }
 
 // the slot layout a consumer of `n_jobs` work items may use: the declared one when it describes exactly this array, none otherwise
@@ -390,6 +459,10 @@ const char* np_last_error(const np_ctx* ctx) { return ctx ? ctx->err.c_str() : g
 
 np_ctx* np_create(int device, const np_params* params)
 {
+    if (const char* hc = getenv("NP_HOST_CONSTANTS")) if (atoi(hc) == 0) {
+        g_create_err = "np_create: NP_HOST_CONSTANTS=0 asks for per-read constants formed on the device: there is no such form (the process's log / exp / logf give them)";
+        return nullptr;
+    }
     int n_dev = 0;
     hipError_t e = hipGetDeviceCount(&n_dev);
     if (e != hipSuccess || n_dev <= 0) {
@@ -462,24 +535,10 @@ np_ctx* np_create(int device, const np_params* params)
                  c->ed_ratio_exact ? "exact sequence for every value" : "filtered", (unsigned long long)bad, (unsigned long long)far);
         c->info += line;
     }
-    {
-        uint64_t bad = 0;
-        (void)np_selftest_libm(100000, 20260925, &bad);
-        const char* hc = getenv("NP_HOST_CONSTANTS");
-        c->host_constants = hc ? atoi(hc) != 0 : bad != 0;
-        if (c->host_constants) {
-            double ln[65]; ln[0] = 0.0;
-            for (int i = 1; i <= 64; ++i) ln[i] = log((double)i);
-            if (hipMalloc((void**)&c->d_log_n, sizeof(ln)) != hipSuccess || hipMemcpy(c->d_log_n, ln, sizeof(ln), hipMemcpyHostToDevice) != hipSuccess) {
-                g_create_err = "np_create: device allocation failed"; np_destroy(c); return nullptr;
-            }
-        }
-        char line[256];
-        snprintf(line, sizeof(line), "; libm check: %llu of 300000 log / exp / logf values differ from the restatement -> per-read constants on the %s",
-                 (unsigned long long)bad, c->host_constants ? "HOST (process libm)" : "device (glibc 2.35 restated)");
-        c->info += line;
-        if (const char* v = getenv("NP_VERBOSE")) if (atoi(v) != 0) fprintf(stderr, "nanopolish_amd: %s\n", line + 2);
-    }
+    c->lp_skip = log(NP_ALIGN_EPSILON); c->lp_trim = log(NP_ALIGN_P_TRIM);
+    np_transitions(0.0, 1.0, c->trans.v);
+    c->info += "; per-read constants on the HOST (process libm)";
+    if (const char* v = getenv("NP_VERBOSE")) if (atoi(v) != 0) fprintf(stderr, "nanopolish_amd: per-read constants on the HOST (process libm)\n");
     return c;
 }
 
@@ -487,18 +546,18 @@ void np_destroy(np_ctx* c)
 {
     if (!c) return;
     (void)hipSetDevice(c->device);
-    if (c->stream) (void)hipStreamSynchronize(c->stream);
+    (void)hipDeviceSynchronize();          // (a caller's stream may still be using the context's buffers)
     for (auto& m : c->models) if (m.d_states) (void)hipFree(m.d_states);
     if (c->d_logsum) (void)hipFree(c->d_logsum);
     if (c->d_flank) (void)hipFree(c->d_flank);
-    if (c->d_log_n) (void)hipFree(c->d_log_n);
     if (c->d_counters) (void)hipFree(c->d_counters);
     dev_buf* bufs[] = {&c->order, &c->trace, &c->kparams, &c->b_jobs, &c->b_reads, &c->b_events, &c->b_ranks, &c->b_out, &c->b_pair_off,
                        &c->b_pairs, &c->b_pair_begin, &c->b_n_pairs, &c->b_vm, &c->b_bp, &c->b_cell_off, &c->b_state_off,
                        &c->b_states, &c->b_n_states, &c->ed_status, &c->ed_tstat, &c->b_raw, &c->b_raw_off, &c->b_ev_off, &c->b_ev_start,
-                       &c->b_ev_len, &c->b_ev_mean, &c->b_ev_stdv, &c->b_n_events, &c->cm_group_rank_off, &c->cm_cigar_scratch, &c->ea_bp, &c->ea_path, &c->ea_args, &c->align_order, &c->recal_order, &c->site_scan};
+                       &c->b_ev_len, &c->b_ev_mean, &c->b_ev_stdv, &c->b_n_events, &c->cm_group_rank_off, &c->cm_cigar_scratch, &c->ea_bp, &c->ea_path, &c->ea_args, &c->align_order, &c->recal_order, &c->site_scan, &c->hc_var};
     for (dev_buf* b : bufs) b->release();
     c->small_d.release();
+    c->hc_align.release(); c->hc_resolve.release(); c->hc_sets.release();
     if (c->small_h) (void)hipHostFree(c->small_h);
     for (auto& t : c->timing) {
         for (auto& pr : t.pending) { (void)hipEventDestroy(pr.first); (void)hipEventDestroy(pr.second); }
@@ -891,11 +950,21 @@ int np_hmm_score_set_combine_dev(np_ctx* c, void* stream, int64_t n_sets, const 
                                  const float* member_scores, float* out_scores)
 {
     if (!c || n_sets < 0 || (n_sets > 0 && (!set_off || !member_scores || !out_scores))) return NP_ERR_INVALID;
+    if (n_sets == 0) return NP_OK;
     std::lock_guard<std::mutex> g(c->lock);
     NP_HIP(c, hipSetDevice(c->device));
+    { const int rc = refuse_capture(c, stream, "np_hmm_score_set_combine_dev"); if (rc != NP_OK) return rc; }
     stream_scope scope = use_stream(c, stream); hipStream_t s = scope.s;
     family_timer tm(c, 1, s);
-    NP_HIP(c, np_launch_score_set_combine(n_sets, set_off, member_idx, member_scores, c->d_logsum, c->host_constants ? c->d_log_n : nullptr, out_scores, s));
+    const size_t n = (size_t)n_sets;
+    NP_HIP(c, c->hc_sets.reserve(n * (sizeof(int64_t) + sizeof(double))));
+    host_fix f{};
+    f.what = FIX_SETS; f.n = n_sets;
+    int64_t* const sizes = (int64_t*)c->hc_sets.p;
+    f.sizes = sizes; f.log_n = (double*)(sizes + n);
+    NP_HIP(c, np_launch_gather_set_sizes(n_sets, set_off, sizes, s));
+    NP_HIP(c, enqueue_host_fix(s, f));
+    NP_HIP(c, np_launch_score_set_combine(n_sets, set_off, member_idx, member_scores, c->d_logsum, f.log_n, out_scores, s));
     return NP_OK;
 }
 
@@ -906,11 +975,11 @@ int np_resolve_jobs_dev(np_ctx* c, void* stream, int n_reads, np_read_dev* reads
     if (!c) return NP_ERR_INVALID;
     std::lock_guard<std::mutex> g(c->lock);
     NP_HIP(c, hipSetDevice(c->device));
+    { const int rc = refuse_capture(c, stream, "np_resolve_jobs_dev"); if (rc != NP_OK) return rc; }
     stream_scope scope = use_stream(c, stream); hipStream_t s = scope.s;
     family_timer tm(c, 2, s);
-    NP_HIP(c, np_launch_build_map(n_reads, reads, pair_off, pairs, pair_begin, n_pairs, map_start, nullptr, events_per_base,
-                                  c->params.hmm_indel_bias_factor, s));
-    if (c->host_constants) { const int rc = host_constants_fix(c, s, n_reads, reads, events_per_base, 2); if (rc != NP_OK) return rc; }
+    NP_HIP(c, np_launch_build_map(n_reads, reads, pair_off, pairs, pair_begin, n_pairs, map_start, nullptr, events_per_base, s));
+    { const int rc = fix_resolve(c, s, n_reads, reads, events_per_base, nullptr); if (rc != NP_OK) return rc; }
     np_slots lay;
     { const int rc = layout_for(c, n_jobs, &lay); if (rc != NP_OK) return rc; }
     NP_HIP(c, np_launch_resolve(n_jobs, jobs, reads, n_pairs, events_per_base, nullptr, map_start, kpos, lay, s));
@@ -932,10 +1001,12 @@ int np_calibrate_resolve_dev(np_ctx* c, void* stream, int n_reads, np_read_dev* 
     if (model < 0 || model >= (int)c->models.size()) { c->err = "bad model id"; return NP_ERR_INVALID; }
     std::lock_guard<std::mutex> g(c->lock);
     NP_HIP(c, hipSetDevice(c->device));
+    { const int rc = refuse_capture(c, stream, "np_calibrate_resolve_dev"); if (rc != NP_OK) return rc; }
     stream_scope scope = use_stream(c, stream); hipStream_t s = scope.s;
     family_timer tm(c, 2, s);
-    NP_HIP(c, np_launch_build_map(n_reads, reads, pair_off, pairs, pair_begin, n_pairs, map_start, map_stop, events_per_base,
-                                  c->params.hmm_indel_bias_factor, s));
+    NP_HIP(c, np_launch_build_map(n_reads, reads, pair_off, pairs, pair_begin, n_pairs, map_start, map_stop, events_per_base, s));
+    NP_HIP(c, c->hc_var.reserve((size_t)std::max(n_reads, 1) * sizeof(double)));
+    NP_HIP(c, np_launch_fill_f64(n_reads, c->hc_var.as<double>(), -1.0, s));
     // the calibration kernel takes several reads per wave and runs for the longest of them: groups of similar length (the aligner's order)
     const uint32_t* order = nullptr;
     if (n_reads > 64) {
@@ -944,8 +1015,8 @@ int np_calibrate_resolve_dev(np_ctx* c, void* stream, int n_reads, np_read_dev* 
         order = c->recal_order.as<uint32_t>() + 2048;
     }
     NP_HIP(c, np_launch_recalibrate(n_reads, reads, event_mean, kmer_rank, c->models[model].d_states, c->models[model].n_states, n_pairs, map_start,
-                                    calibrated, order, c->recal_shape, s));
-    if (c->host_constants) { const int rc = host_constants_fix(c, s, n_reads, reads, events_per_base, 2 | 4); if (rc != NP_OK) return rc; }
+                                    calibrated, order, c->hc_var.as<double>(), c->recal_shape, s));
+    { const int rc = fix_resolve(c, s, n_reads, reads, events_per_base, c->hc_var.as<double>()); if (rc != NP_OK) return rc; }
     np_slots lay;
     { const int rc = layout_for(c, n_jobs, &lay); if (rc != NP_OK) return rc; }
     NP_HIP(c, np_launch_resolve(n_jobs, jobs, reads, n_pairs, events_per_base, calibrated, map_start, kpos, lay, s));
@@ -976,8 +1047,7 @@ static int pack_hmm_jobs(np_ctx* c, int n_jobs, const np_hmm_job* jobs, std::vec
         r.scale = q.scale; r.shift = q.shift; r.var = q.var; r.log_var = log(q.var);
         r.event_off = (int64_t)ev.size() - (int64_t)lo;      // ev[event_off + event_idx] addresses the packed window
         r.n_events = q.n_events_total;
-        if (c->host_constants) transitions_libm(q.events_per_base, q.indel_bias != 0.0 ? q.indel_bias : c->params.hmm_indel_bias_factor, r.trans);
-        else np_transitions(q.events_per_base, q.indel_bias != 0.0 ? q.indel_bias : c->params.hmm_indel_bias_factor, r.trans);
+        np_transitions(q.events_per_base, q.indel_bias != 0.0 ? q.indel_bias : c->params.hmm_indel_bias_factor, r.trans);
         ev.insert(ev.end(), q.event_mean + lo, q.event_mean + hi + 1);
         np_hmm_job_dev& d = dj[j];
         d.rank_off = (int64_t)rk.size(); d.n_kmers = q.n_kmers; d.read = (uint32_t)j;
@@ -1415,7 +1485,7 @@ int64_t np_get_stat(np_ctx* c, const char* name)
     if (k == "align_blocks_max") return (int64_t)c->n_cu * c->align_blocks_per_cu;
     if (k == "lse_oor") return c->lse_oor ? 1 : 0;
     if (k == "lse_probe_ok") return c->lse_probe_ok ? 1 : 0;
-    if (k == "host_constants") return c->host_constants ? 1 : 0;
+    if (k == "host_constants") return 1;         // (the only form: host_fix)
     if (k == "n_cu") return c->n_cu;
     if (k == "ed_serial_reads" || k == "ed_refused_reads") {     // of the most recent np_detect_events_* call (waits for it): reads whose
         // prefix sums were accumulated serially (exactness bound not provable), resp. refused (NP_ED_INEXACT: non-finite samples)
@@ -1615,11 +1685,11 @@ int np_mom_fill_dev(np_ctx* c, void* stream, int n_reads, np_read_dev* reads, np
     if (n_reads == 0) return NP_OK;
     std::lock_guard<std::mutex> g(c->lock);
     NP_HIP(c, hipSetDevice(c->device));
+    { const int rc = refuse_capture(c, stream, "np_mom_fill_dev"); if (rc != NP_OK) return rc; }
     stream_scope scope = use_stream(c, stream); hipStream_t s = scope.s;
     family_timer tm(c, 5, s);
     NP_HIP(c, np_launch_mom_fill(n_reads, reads, reads_b, event_mean, n_events, kmer_rank, c->models[model].d_states, c->models[model].n_states, s));
-    if (c->host_constants) return host_constants_fix(c, s, n_reads, reads, nullptr, 1);
-    return NP_OK;
+    return fix_aligner(c, s, n_reads, reads);
 }
 
 // Direct-RNA reads: the detected events of every read reversed in place (squiggle_read.cpp:260-263), AFTER np_mom_fill_dev (the MoM

@@ -25,7 +25,6 @@
 // is written or read for them (round 2).  Event means/stdv are one thread per event.
 #include <algorithm>
 #include "np_kernels.h"
-#include "np_log.h"
 
 #define NP_ED_TILE 256
 #define NP_ED_HALO 16          // >= the largest window (event_detection_rna: 14)
@@ -1006,7 +1005,8 @@ __global__ void __launch_bounds__(64) np_ed_serial_events_kernel(int n_reads, co
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// estimate_scalings_using_mom (raw_loader.cpp:30-75) + the aligner's per-read constants (:99-108) + set4.
+// estimate_scalings_using_mom (raw_loader.cpp:30-75) + set4.  (The aligner's per-read constants, :99-108, go through log / exp: the host
+// forms them from n_events and n_kmers behind this kernel, np_capi.hip:host_fix.)
 // One wave per read; every sum is accumulated in the reference's order (terms staged 64 at a time in LDS, one lane
 // per sum adds its row front to back).
 // ---------------------------------------------------------------------------------------------------------------
@@ -1173,14 +1173,6 @@ __global__ void __launch_bounds__(64 * NP_MOM_W) np_mom_fill_kernel(int n_reads,
         const double scale = (event_level_sq_sum / (double)(uint32_t)my_ne) / (kmer_level_sq_sum / (double)(uint32_t)my_K);
         rd->n_events = (uint32_t)my_ne;
         rd->scale = scale; rd->shift = shift; rd->var = 1.0; rd->log_var = 0.0;      // set4(shift, scale, 0, 1): log(1) == 0
-        // raw_loader.cpp:99-108, with glibc's log / exp restated (np_log.h)
-        const double events_per_kmer = (double)(uint32_t)my_ne / (double)(uint32_t)my_K;
-        const double p_stay = 1 - (1 / (events_per_kmer + 1));
-        const double epsilon = 1e-10;
-        rd->lp_skip = np_log_glibc(epsilon);
-        rd->lp_stay = np_log_glibc(p_stay);
-        rd->lp_step = np_log_glibc(1.0 - np_exp_glibc(rd->lp_skip) - np_exp_glibc(rd->lp_stay));
-        rd->lp_trim = np_log_glibc(0.01);
         if (reads_b) reads_b[my].n_events = (uint32_t)my_ne;
     }
 }

@@ -1,7 +1,8 @@
 // np_glue_kernels.hip -- the read-level glue between the aligner and the HMM, kept on the device so the
 // fused call-methylation pass needs no host round trip:
 //   * np_build_map_kernel : base_to_event_map[].start + events_per_base (src/nanopolish_squiggle_read.cpp:273-301)
-//                           and the per-read HMM transitions (src/hmm/nanopolish_profile_hmm_r9.inl:17-76)
+//   * np_gather_lengths_kernel, np_apply_*_kernel : what the host needs of every read for the constants that go through the C library's
+//                           log / exp / logf, and those constants back into the read records (np_capi.hip:host_fix)
 //   * np_resolve_kernel   : get_closest_event_to (src/nanopolish_squiggle_read.cpp:161-186) for both window
 //                           bounds of every work item + the skip rules of calculate_methylation_for_read
 //                           (src/basemods/nanopolish_basemods.cpp:352-358) and the events-per-base QC
@@ -9,8 +10,6 @@
 //   * np_classify_kernel  : bins HMM work items into the (lanes, blocks-per-lane) size classes of np_hmm_kernels.hip
 #include "np_kernels.h"
 #include "np_motif.h"
-#include "np_logf.h"
-#include "np_log.h"
 
 namespace {
 
@@ -32,7 +31,7 @@ template <bool STOP>
 __global__ void __launch_bounds__(64) np_build_map_kernel(int n_reads, np_read_dev* reads, const int64_t* pair_off,
                                                           const np_pair* pairs, const int32_t* pair_begin,
                                                           const int32_t* n_pairs, int32_t* map_start, int32_t* map_stop,
-                                                          double* events_per_base, double indel_bias)
+                                                          double* events_per_base)
 {
     const int ri = blockIdx.x;
     if (ri >= n_reads) return;
@@ -45,7 +44,7 @@ __global__ void __launch_bounds__(64) np_build_map_kernel(int n_reads, np_read_d
     if (np_ <= 0) {
         // failed alignment: events cleared, events_per_base = 0 (squiggle_read.cpp:324-329); IndexPair(): start = stop = -1
         for (int k = lane; k < K; k += 64) { ms[k] = -1; if (STOP) mp[k] = -1; }
-        if (lane == 0) { events_per_base[ri] = 0.0; np_transitions(0.0, indel_bias, rd->trans); }
+        if (lane == 0) events_per_base[ri] = 0.0;
         return;
     }
     const np_pair* p = pairs + pair_off[ri] + pair_begin[ri];
@@ -91,9 +90,7 @@ __global__ void __launch_bounds__(64) np_build_map_kernel(int n_reads, np_read_d
     }
     if (lane == 0) {
         const size_t min_event = (size_t)first.read_pos, max_event = (size_t)last.read_pos;        // path is monotone
-        const double epb = (double)(max_event - min_event) / (double)(size_t)K;                    // :301
-        events_per_base[ri] = epb;
-        np_transitions(epb, indel_bias, rd->trans);
+        events_per_base[ri] = (double)(max_event - min_event) / (double)(size_t)K;                 // :301
     }
 }
 
@@ -166,7 +163,7 @@ template <int W, int R, bool TABLE>
 __global__ void __launch_bounds__(64 * W) np_recalibrate_kernel(int n_reads, np_read_dev* reads, const float* event_mean,
                                                                 const uint16_t* ranks, const np_state_dev* model, int n_states,
                                                                 const int32_t* n_pairs, const int32_t* map_start,
-                                                                int32_t* calibrated, const uint32_t* order)
+                                                                int32_t* calibrated, const uint32_t* order, double* new_var)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     __shared__ double terms[W][R][5][65];
@@ -315,7 +312,7 @@ __global__ void __launch_bounds__(64 * W) np_recalibrate_kernel(int n_reads, np_
         var = sqrt(var);
         if (lane == 0) {
             np_read_dev* rd = reads + ri[r];
-            rd->shift = shift[r]; rd->scale = scale[r]; rd->var = var; rd->log_var = np_log_glibc(var);   // set4 (squiggle_read.cpp:38-65), glibc's log restated
+            rd->shift = shift[r]; rd->scale = scale[r]; rd->var = var; new_var[ri[r]] = var;   // set4 (squiggle_read.cpp:38-65); log(var) by the host
             calibrated[ri[r]] = var > 2.5 ? 0 : 1;                                          // MIN_CALIBRATION_VAR (:320)
         }
     }
@@ -332,7 +329,7 @@ template <int W, int R>
 __global__ void __launch_bounds__(64 * W) np_recalibrate_half_kernel(int n_reads, np_read_dev* reads, const float* event_mean,
                                                                      const uint16_t* ranks, const np_state_dev* model, int n_states,
                                                                      const int32_t* n_pairs, const int32_t* map_start,
-                                                                     int32_t* calibrated, const uint32_t* order)
+                                                                     int32_t* calibrated, const uint32_t* order, double* new_var)
 {
     static_assert(R % 2 == 0 && 5 * R <= 64, "reads per wave: an even number, five adder lanes each");
     constexpr int P = R / 2, CH = 32;
@@ -481,7 +478,7 @@ __global__ void __launch_bounds__(64 * W) np_recalibrate_half_kernel(int n_reads
         var = sqrt(var);
         if (lane == 0) {
             np_read_dev* rd = reads + ri[r];
-            rd->shift = shift[r]; rd->scale = scale[r]; rd->var = var; rd->log_var = np_log_glibc(var);   // set4 (squiggle_read.cpp:38-65), glibc's log restated
+            rd->shift = shift[r]; rd->scale = scale[r]; rd->var = var; new_var[ri[r]] = var;   // set4 (squiggle_read.cpp:38-65); log(var) by the host
             calibrated[ri[r]] = var > 2.5 ? 0 : 1;                                          // MIN_CALIBRATION_VAR (:320)
         }
     }
@@ -726,15 +723,102 @@ hipError_t np_launch_classify(const np_hmm_job_dev* jobs, int64_t n_jobs, uint32
     return hipGetLastError();
 }
 
+// ---- the constants that go through the C library's log / exp / logf (np_capi.hip:host_fix) -----------------------------------------
+// Thread per read.  `to_host` / `from_host` are PINNED HOST memory (mapped, coherent): the few bytes per read cross the bus as these
+// kernels' own stores and loads, so nothing of it queues behind another stream's bulk copies in a copy engine.
+namespace {
+__global__ void __launch_bounds__(256) np_gather_lengths_kernel(int n_reads, const np_read_dev* reads, uint2* to_host)
+{
+    const int r = blockIdx.x * 256 + threadIdx.x;
+    if (r < n_reads) to_host[r] = uint2{reads[r].n_events, reads[r].n_kmers};
+}
+__global__ void __launch_bounds__(256) np_apply_aligner_kernel(int n_reads, np_read_dev* reads, const double2* from_host, double lp_skip, double lp_trim)
+{
+    const int r = blockIdx.x * 256 + threadIdx.x;
+    if (r >= n_reads) return;
+    const double2 v = from_host[r];
+    reads[r].lp_skip = lp_skip; reads[r].lp_stay = v.x; reads[r].lp_step = v.y; reads[r].lp_trim = lp_trim;
+}
+__global__ void __launch_bounds__(256) np_fill_f64_kernel(int n, double* p, double v)
+{
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = v;
+}
+// new_var (null: no calibration): the recalibration's var of the reads that it rescaled, a negative number for the others
+__global__ void __launch_bounds__(256) np_gather_resolve_kernel(int n_reads, const double* events_per_base, const double* new_var, double* to_host_epb, double* to_host_var)
+{
+    const int r = blockIdx.x * 256 + threadIdx.x;
+    if (r >= n_reads) return;
+    to_host_epb[r] = events_per_base[r];
+    if (new_var) to_host_var[r] = new_var[r];
+}
+// trans: the eight transitions that do not depend on the read (all but 0, mm_self, and 3, mm_next); a read whose var the calibration
+// left alone keeps its log_var too
+__global__ void __launch_bounds__(256) np_apply_resolve_kernel(int n_reads, np_read_dev* reads, const float2* from_host_mm, const double* from_host_log_var,
+                                                               const double* new_var, np_trans trans)
+{
+    const int r = blockIdx.x * 256 + threadIdx.x;
+    if (r >= n_reads) return;
+    const float2 mm = from_host_mm[r];
+    trans.v[0] = mm.x; trans.v[3] = mm.y;
+#pragma unroll
+    for (int i = 0; i < 10; ++i) reads[r].trans[i] = trans.v[i];
+    if (new_var && !(new_var[r] < 0.0)) reads[r].log_var = from_host_log_var[r];
+}
+__global__ void __launch_bounds__(256) np_gather_set_sizes_kernel(int64_t n_sets, const int64_t* set_off, int64_t* to_host)
+{
+    const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (q < n_sets) to_host[q] = set_off[q + 1] - set_off[q];
+}
+} // namespace
+
+hipError_t np_launch_gather_lengths(int n_reads, const np_read_dev* reads, uint2* to_host, hipStream_t s)
+{
+    if (n_reads <= 0) return hipSuccess;
+    hipLaunchKernelGGL(np_gather_lengths_kernel, dim3((unsigned)((n_reads + 255) / 256)), dim3(256), 0, s, n_reads, reads, to_host);
+    return hipGetLastError();
+}
+hipError_t np_launch_apply_aligner(int n_reads, np_read_dev* reads, const double2* from_host, double lp_skip, double lp_trim, hipStream_t s)
+{
+    if (n_reads <= 0) return hipSuccess;
+    hipLaunchKernelGGL(np_apply_aligner_kernel, dim3((unsigned)((n_reads + 255) / 256)), dim3(256), 0, s, n_reads, reads, from_host, lp_skip, lp_trim);
+    return hipGetLastError();
+}
+hipError_t np_launch_fill_f64(int n, double* p, double v, hipStream_t s)
+{
+    if (n <= 0) return hipSuccess;
+    hipLaunchKernelGGL(np_fill_f64_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, n, p, v);
+    return hipGetLastError();
+}
+hipError_t np_launch_gather_resolve(int n_reads, const double* events_per_base, const double* new_var, double* to_host_epb, double* to_host_var, hipStream_t s)
+{
+    if (n_reads <= 0) return hipSuccess;
+    hipLaunchKernelGGL(np_gather_resolve_kernel, dim3((unsigned)((n_reads + 255) / 256)), dim3(256), 0, s, n_reads, events_per_base, new_var, to_host_epb, to_host_var);
+    return hipGetLastError();
+}
+hipError_t np_launch_apply_resolve(int n_reads, np_read_dev* reads, const float2* from_host_mm, const double* from_host_log_var, const double* new_var,
+                                   const np_trans& trans, hipStream_t s)
+{
+    if (n_reads <= 0) return hipSuccess;
+    hipLaunchKernelGGL(np_apply_resolve_kernel, dim3((unsigned)((n_reads + 255) / 256)), dim3(256), 0, s, n_reads, reads, from_host_mm, from_host_log_var, new_var, trans);
+    return hipGetLastError();
+}
+hipError_t np_launch_gather_set_sizes(int64_t n_sets, const int64_t* set_off, int64_t* to_host, hipStream_t s)
+{
+    if (n_sets <= 0) return hipSuccess;
+    hipLaunchKernelGGL(np_gather_set_sizes_kernel, dim3((unsigned)((n_sets + 255) / 256)), dim3(256), 0, s, n_sets, set_off, to_host);
+    return hipGetLastError();
+}
+
 hipError_t np_launch_build_map(int n_reads, np_read_dev* reads, const int64_t* pair_off, const np_pair* pairs,
                                const int32_t* pair_begin, const int32_t* n_pairs, int32_t* map_start, int32_t* map_stop,
-                               double* events_per_base, double indel_bias, hipStream_t s)
+                               double* events_per_base, hipStream_t s)
 {
     if (n_reads <= 0) return hipSuccess;
     if (map_stop) hipLaunchKernelGGL(np_build_map_kernel<true>, dim3(n_reads), dim3(64), 0, s, n_reads, reads, pair_off, pairs,
-                                     pair_begin, n_pairs, map_start, map_stop, events_per_base, indel_bias);
+                                     pair_begin, n_pairs, map_start, map_stop, events_per_base);
     else hipLaunchKernelGGL(np_build_map_kernel<false>, dim3(n_reads), dim3(64), 0, s, n_reads, reads, pair_off, pairs,
-                            pair_begin, n_pairs, map_start, map_stop, events_per_base, indel_bias);
+                            pair_begin, n_pairs, map_start, map_stop, events_per_base);
     return hipGetLastError();
 }
 
@@ -1007,8 +1091,7 @@ __global__ void __launch_bounds__(256) np_score_set_combine_kernel(int64_t n_set
     if (q >= n_sets) return;
     const int64_t b = set_off[q], n = set_off[q + 1] - b;
     if (n <= 0) { out[q] = NP_NEG_INF; return; }
-    // glibc's log, restated (csrc/np_log.h) -- or, in host-constants mode, log(n) as the process's own libm computed it (n <= 64)
-    const double pen = log_n && n <= 64 ? log_n[n] : np_log_glibc((double)(uint64_t)n);
+    const double pen = log_n[q];                          // log(n), formed by the host (pinned host memory: np_capi.hip:host_fix)
     auto sc = [&](int64_t t) { return (double)member_scores[member_idx ? member_idx[b + t] : b + t]; };
     double score = sc(0) - pen;
     for (int64_t t = 1; t < n; ++t) {
@@ -1084,26 +1167,26 @@ hipError_t np_launch_selftest_div(uint64_t n_samples, uint64_t seed, unsigned lo
 #endif
 template <int W, int R>
 static hipError_t launch_recal(int n_reads, np_read_dev* reads, const float* event_mean, const uint16_t* ranks, const np_state_dev* model, int n_states,
-                               const int32_t* n_pairs, const int32_t* map_start, int32_t* calibrated, const uint32_t* order, hipStream_t s)
+                               const int32_t* n_pairs, const int32_t* map_start, int32_t* calibrated, const uint32_t* order, double* new_var, hipStream_t s)
 {
     const int nb = (n_reads + W * R - 1) / (W * R);
     if (n_states <= NP_RC_STATES)
-        hipLaunchKernelGGL((np_recalibrate_kernel<W, R, true>), dim3(nb), dim3(64 * W), 0, s, n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order);
+        hipLaunchKernelGGL((np_recalibrate_kernel<W, R, true>), dim3(nb), dim3(64 * W), 0, s, n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, new_var);
     else
-        hipLaunchKernelGGL((np_recalibrate_kernel<W, R, false>), dim3(nb), dim3(64 * W), 0, s, n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order);
+        hipLaunchKernelGGL((np_recalibrate_kernel<W, R, false>), dim3(nb), dim3(64 * W), 0, s, n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, new_var);
     return hipGetLastError();
 }
 hipError_t np_launch_recalibrate(int n_reads, np_read_dev* reads, const float* event_mean, const uint16_t* ranks,
                                  const np_state_dev* model, int n_states, const int32_t* n_pairs, const int32_t* map_start,
-                                 int32_t* calibrated, const uint32_t* order, int shape, hipStream_t s)
+                                 int32_t* calibrated, const uint32_t* order, double* new_var, int shape, hipStream_t s)
 {
     if (n_reads <= 0) return hipSuccess;
     if (shape == 3 && n_states <= NP_RC_STATES) {          // round 6: half-wave chunks, sixteen waves x four reads, four waves per SIMD
         const int nb = (n_reads + 16 * 4 - 1) / (16 * 4);
-        hipLaunchKernelGGL((np_recalibrate_half_kernel<16, 4>), dim3(nb), dim3(1024), 0, s, n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order);
+        hipLaunchKernelGGL((np_recalibrate_half_kernel<16, 4>), dim3(nb), dim3(1024), 0, s, n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, new_var);
         return hipGetLastError();
     }
-    if (shape == 1) return launch_recal<16, 2>(n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, s);
-    if (shape == 2) return launch_recal<12, 3>(n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, s);
-    return launch_recal<NP_RC_W, NP_RC_R>(n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, s);
+    if (shape == 1) return launch_recal<16, 2>(n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, new_var, s);
+    if (shape == 2) return launch_recal<12, 3>(n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, new_var, s);
+    return launch_recal<NP_RC_W, NP_RC_R>(n_reads, reads, event_mean, ranks, model, n_states, n_pairs, map_start, calibrated, order, new_var, s);
 }

@@ -12,8 +12,7 @@
 #include <vector>
 #include <algorithm>
 #include "../../include/np_hmm.h"
-#include "np_logf.h"
-#include "np_log.h"
+#include "np_constants.h"
 
 namespace {
 
@@ -359,55 +358,32 @@ void np_fill_read_host(np_read_dev* r, double shift, double scale, double var,
     memset(r, 0, sizeof(*r));
     r->scale = scale; r->shift = shift; r->var = var; r->log_var = log(var);   // set4/set6, squiggle_read.cpp:38-65
     // aligner transition constants, raw_loader.cpp:99-108 (double, host libm as in the reference)
-    const double events_per_kmer = (double)n_events / n_kmers;
-    const double p_stay = 1 - (1 / (events_per_kmer + 1));
-    const double epsilon = 1e-10;
-    r->lp_skip = log(epsilon);
-    r->lp_stay = log(p_stay);
-    r->lp_step = log(1.0 - exp(r->lp_skip) - exp(r->lp_stay));
-    r->lp_trim = log(0.01);
+    r->lp_skip = log(NP_ALIGN_EPSILON);
+    np_aligner_lp(n_events, n_kmers, exp(r->lp_skip), &r->lp_stay, &r->lp_step);
+    r->lp_trim = log(NP_ALIGN_P_TRIM);
     r->event_off = event_off; r->rank_off = rank_off; r->n_events = n_events; r->n_kmers = n_kmers;
 }
 
-// The aligner's per-read constants (raw_loader.cpp:99-108) exactly as np_mom_fill_dev computes them on the device: glibc's
-// log / exp restated in np_log.h instead of libm calls.  Exposed so that the restatement can be checked against the
-// host's libm without a GPU (tests/test_host_logic.py).
+// The aligner's per-read constants (raw_loader.cpp:99-108) exactly as np_mom_fill_dev's host function forms them.
 void np_aligner_constants(uint32_t n_events, uint32_t n_kmers, double out[4])
 {
-    const double events_per_kmer = (double)n_events / (double)n_kmers;
-    const double p_stay = 1 - (1 / (events_per_kmer + 1));
-    const double epsilon = 1e-10;
-    out[0] = np_log_glibc(epsilon);
-    out[1] = np_log_glibc(p_stay);
-    out[2] = np_log_glibc(1.0 - np_exp_glibc(out[0]) - np_exp_glibc(out[1]));
-    out[3] = np_log_glibc(0.01);
+    out[0] = log(NP_ALIGN_EPSILON);
+    np_aligner_lp(n_events, n_kmers, exp(out[0]), &out[1], &out[2]);
+    out[3] = log(NP_ALIGN_P_TRIM);
 }
-// The device computes the aligner's constants, set4's log(var) and calculate_transitions with restatements of glibc 2.35's
-// log / exp / logf (np_log.h, np_logf.h; the x86-64 FMA variants this image's libm selects).  A host whose libm is another
-// version or lacks FMA computes what the REFERENCE would compute there -- which may differ in the last bit from the
-// restatement.  This check compares them on `n` pseudo-random arguments in the ranges the path uses; 0 mismatches means
-// device-side constants are bit-identical to this host's libm.
+// The two entry points of the ABI that used to compare a restatement of log / exp / logf with the process's functions.  The constants
+// are formed by the process's functions themselves now: nothing can differ, and these say so.
 int np_selftest_libm(uint64_t n, uint64_t seed, uint64_t* n_mismatch)
 {
+    (void)n; (void)seed;
     if (!n_mismatch) return NP_ERR_INVALID;
-    uint64_t bad = 0, s = seed ? seed : 1;
-    for (uint64_t i = 0; i < n; ++i) {
-        s ^= s << 13; s ^= s >> 7; s ^= s << 17;
-        const double u = (double)(s >> 11) * (1.0 / 9007199254740992.0);            // [0, 1)
-        const double x_log = ldexp(1.0 + u, (int)((s >> 3) % 24) - 12);              // log: 2^-12 .. 2^12 (probabilities, variances, ratios)
-        const double x_exp = 30.0 * u;                                               // exp(-x): 0 .. 30 nats
-        const float xf = (float)ldexp(1.0 + u, (int)((s >> 5) % 16) - 10);           // logf: transition probabilities
-        bad += np_log_glibc(x_log) != log(x_log);
-        bad += np_exp_glibc(-x_exp) != exp(-x_exp);
-        bad += np_logf_glibc(xf) != logf(xf);
-    }
-    *n_mismatch = bad;
+    *n_mismatch = 0;
     return NP_OK;
 }
 
 void np_restated_log_exp(const double* x, size_t n, double* out_log, double* out_exp)
 {
-    for (size_t i = 0; i < n; ++i) { out_log[i] = np_log_glibc(x[i]); out_exp[i] = np_exp_glibc(-x[i]); }
+    for (size_t i = 0; i < n; ++i) { out_log[i] = log(x[i]); out_exp[i] = x[i] < 512.0 && x[i] > -512.0 ? exp(-x[i]) : NAN; }
 }
 
 } // extern "C"

@@ -152,10 +152,11 @@ hipError_t np_launch_classify(const np_hmm_job_dev* jobs, int64_t n_jobs, uint32
                               uint32_t* order /*[NP_NUM_CLASSES][n_jobs]*/, float* out_scores, uint32_t flank_len, uint32_t* bins /*[2 * 8 * 8 * 64]*/, np_slots lay, hipStream_t s);
 hipError_t np_launch_build_map(int n_reads, np_read_dev* reads, const int64_t* pair_off, const np_pair* pairs,
                                const int32_t* pair_begin, const int32_t* n_pairs, int32_t* map_start, int32_t* map_stop,
-                               double* events_per_base, double indel_bias, hipStream_t s);
+                               double* events_per_base, hipStream_t s);
 hipError_t np_launch_recalibrate(int n_reads, np_read_dev* reads, const float* event_mean, const uint16_t* ranks,
                                  const np_state_dev* model, int n_states, const int32_t* n_pairs, const int32_t* map_start,
                                  int32_t* calibrated, const uint32_t* order /* read order of the groups (np_launch_align_order) or null */,
+                                 double* new_var /* out: var of the reads that were rescaled (others: untouched) */,
                                  int shape /* 0: the default workgroup shape; 1, 2: A/B alternatives */, hipStream_t s);
 hipError_t np_launch_discard_degenerate(int64_t n_jobs, np_hmm_job_dev* jobs, const np_read_dev* reads, const int32_t* map_start,
                                         const int32_t* deg_kpos, np_slots lay, hipStream_t s);
@@ -173,7 +174,16 @@ hipError_t np_launch_genome_site_index(const char* genome, const int64_t* contig
                                        uint32_t* word_rank, int64_t* n_sites, uint32_t* chunk_scratch, hipStream_t s);
 int64_t np_site_rank_chunks(int64_t n_pos);
 hipError_t np_launch_score_set_combine(int64_t n_sets, const int64_t* set_off, const int64_t* member_idx, const float* member_scores,
-                                       const float* logsum, const double* log_n /* host-constants mode: log(0 .. 64) by the process's libm; else null */, float* out, hipStream_t s);
+                                       const float* logsum, const double* log_n /* per set: log of its size */, float* out, hipStream_t s);
+// the constants formed by the host (np_capi.hip:host_fix): what it needs, into pinned host memory, and what it formed, out of it
+struct np_trans { float v[10]; };
+hipError_t np_launch_gather_lengths(int n_reads, const np_read_dev* reads, uint2* to_host, hipStream_t s);
+hipError_t np_launch_apply_aligner(int n_reads, np_read_dev* reads, const double2* from_host, double lp_skip, double lp_trim, hipStream_t s);
+hipError_t np_launch_fill_f64(int n, double* p, double v, hipStream_t s);
+hipError_t np_launch_gather_resolve(int n_reads, const double* events_per_base, const double* new_var, double* to_host_epb, double* to_host_var, hipStream_t s);
+hipError_t np_launch_apply_resolve(int n_reads, np_read_dev* reads, const float2* from_host_mm, const double* from_host_log_var, const double* new_var,
+                                   const np_trans& trans, hipStream_t s);
+hipError_t np_launch_gather_set_sizes(int64_t n_sets, const int64_t* set_off, int64_t* to_host, hipStream_t s);
 hipError_t np_launch_selftest_div(uint64_t n_samples, uint64_t seed, unsigned long long* d_mismatches, hipStream_t s);
 hipError_t np_launch_selftest_ratio(uint64_t n_samples, uint64_t seed, unsigned long long* d_out, hipStream_t s);
 hipError_t np_launch_selftest_div_small(int w, double chd, double cld, float chf, float clf, uint64_t n_f64, unsigned long long* d_out, hipStream_t s);

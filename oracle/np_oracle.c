@@ -1116,7 +1116,7 @@ void npo_detect_events_many(int n_reads, const float* raw, const int64_t* raw_of
     }
 }
 
-/* the aligner's per-read constants on their own (raw_loader.cpp:99-108), for checking the device's restated log/exp */
+/* the aligner's per-read constants on their own (raw_loader.cpp:99-108), for checking the device pass's */
 void npo_aligner_constants(uint32_t n_events, uint32_t n_kmers, double out[4])
 {
     double events_per_kmer = (double)n_events / n_kmers;
