@@ -10,11 +10,10 @@
 //     "last aligned pair with ref_pos <= x" search), closest events from the read's event map (np_device.h);
 //   * Viterbi fill as an anti-diagonal sweep, two segments (of two reads) per wave, one per half-wave: lane j of a half owns three
 //     k-mer blocks (a segment has <= 96 k-mers; four for the k = 5 model), computes row t - j at step t; previous row in registers,
-//     left neighbour through DPP; candidates in HMMMovementType order, later index wins ties; only back-pointers leave the wave, as
-//     64-bit lane masks (six planes per block: the compares' own result registers) written by scalar stores, one line per sweep STEP
-//     (cell (row r, k-mer b) sits in line r + b / BPL), into a per-wave scratch that stays in L2 (ea_fill2);
-//   * back-track of both halves' segments as vector code over a window of lines staged -- and expanded to per-state move codes -- in LDS,
-//     in bursts of steps whose number is known in advance; the visited states go to a per-half list, one 64-bit word per burst
+//     left neighbour through DPP; candidates in HMMMovementType order, later index wins ties; only back-pointers leave the wave, six
+//     bits per block, one dword per lane and one 256-byte line per sweep STEP (cell (row r, k-mer b) sits in line r + b / BPL, dword
+//     b / BPL of its half), into a per-wave scratch (ea_fill2);
+//   * back-track of both halves' segments as vector code over a window of lines staged in LDS, in bursts of steps whose number is known in advance; the visited states go to a per-half list, one 64-bit word per burst
 //     (ea_walk2); then a lane per burst replays it and emits (ballots + prefix counts reproduce the reference's "first 50 that are not K
 //     and not the start event" cut, ea_emit_segment).
 // Output rows are (ref_position relative to the record's pos, event_idx, state 'M'/'B'); ref_kmer / model_kmer of the TSV
@@ -45,20 +44,19 @@ struct ea_trans { float mm_self, mb, mk, mm_next, bb, bk, bm_next, bm_self, kk, 
 // then for half 1; a half whose read is finished pulls the next read from the queue, a half without work sweeps an empty
 // segment.  The per-read state that survives from segment to segment is ten integers per half (ea_half); what only depends on
 // the read's index is reloaded where it is needed (wave-uniform loads).
-// Back-pointers: one dword per lane and sweep step (nine bits per block, see ea_block), one 256-byte line per step: cell
-// (row r, k-mer b) of half h lives in line r + b / 3, dword 32 h + b / 3, bits 9 (b % 3) .. 9 (b % 3) + 8.
 // ---------------------------------------------------------------------------------------------------------------------------
-// Round 4: the back-pointers of a sweep step leave the wave as 64-bit LANE MASKS (bit planes), six per k-mer block of a lane, written
-// by SCALAR stores, instead of one packed dword per lane (round 3).  Why: a step's vector instructions were 40 % selects and shifts
-// that only turn compare results -- lane masks in scalar registers already -- into per-lane codes (23 v_cndmask + 4 v_or3 of ~122
-// instructions, all in the slow issue class).  The masks ARE the information: per block the M cell's code (3 bits: planes 0-2,
-// combined from the four equality masks by scalar logic, which has an issue port of its own), the B cell's bit (plane 3), the K cell's
-// two (planes 4-5: PREV_K, and PREV_B without PREV_K).  A line is 6 x BPL x 8 bytes (144 at three blocks per lane, round 3: 256); bit
-// l of a plane is lane l's block, so half h's walk reads dword h of a plane.
+// Back-pointers: SIX bits per k-mer block.  The compares' results are lane masks in scalar registers; scalar logic, which has an issue
+// port of its own, turns them into six masks per block, and the lane's word takes one bit of each by an add with carry
+// (x = 2 x + mask bit: one vector instruction per mask):
+//   bits 5..3  the M cell's move code (3 bits)
+//   bit  2     the B cell's: code 1 + bit
+//   bits 1..0  the K cell's: code 4 + bits
+// block c of the lane in bits 6 c .. 6 c + 5 of its dword.  A line is 64 dwords, 256 bytes, one coalesced vector store: half h's walk
+// reads its 128-byte half of a line.
 // BPL, the k-mer blocks per lane: a segment spans up to 101 reference bases (eventalign.cpp:695-735), i.e. 102 - k k-mers: 96 for the
 // DNA models (k = 6: three blocks on each of a half-wave's 32 lanes), 97 for the direct-RNA model (k = 5): that one k-mer more takes a
-// fourth block per lane (np_eventalign_chain2_kernel<WAVES, 4>: the same code, 24 planes per line).
-#define NP_EA2_LINE_BYTES(BPL) (48 * (BPL))
+// fourth block per lane (np_eventalign_chain2_kernel<WAVES, 4>: the same code, 24 bits of the dword).
+#define NP_EA2_LINE_BYTES 256
 #ifndef NP_EA_ARGMAX
 #define NP_EA_ARGMAX 1           // the M cell's arg-max: 0 = tournament (round 3), 1 = three-input maxima + equality chain (round 4)
 #endif
@@ -107,16 +105,12 @@ struct ea_half {                 // chain state of the read a half-wave works on
     int e_start, stride, e, n, last_section;
 };
 
-// one k-mer block of one lattice row: the candidates of r9.inl:130-197 in HMMMovementType order, later index wins ties;
-// (lM_r, lB_r, lK_r): the block to the left in this row, (lM_p, ...): in the previous row.
-// Returns the block's back-pointers as NINE bits, three per state (K in bits 0..2, B in 3..5, M in 6..8), each already the
-// back-track's move: bit 2 = "the k-mer steps back", bits 1..0 = the state walked to (2 MATCH, 1 BAD_EVENT, 0 KMER_SKIP), 7 = soft
-// clip (stop).  I.e. HMT_FROM_SAME_M 2, PREV_M 6, SAME_B 1, PREV_B 5, PREV_K 4, SOFT 7 (r9.cpp:150-186): the walk needs no decoding.
 // One k-mer block of one lattice row (the candidates of r9.inl:130-197 in HMMMovementType order, later index wins ties; (lM_r, lB_r,
 // lK_r): the block to the left in this row, (lM_p, ...): in the previous row) with the back-pointers as lane masks: p[0..2] the M cell's move code bit by bit (HMT_FROM_SAME_M 2, PREV_M 6,
 // SAME_B 1, PREV_B 5, PREV_K 4, SOFT 7: bit 2 = "the k-mer steps back", bits 1..0 = the state walked to, 2 MATCH, 1 BAD_EVENT, 0
-// KMER_SKIP; 7 = soft clip, stop -- r9.cpp:150-186), p[3] "B comes from the block's own B", p[4] "K comes from PREV_K", p[5] "K
-// comes from PREV_B and not from PREV_K" (the walk: B 2 - p3, K 6 - p5 - 2 p4).  The masks are the compares' own result registers;
+// KMER_SKIP; 7 = soft clip, stop -- r9.cpp:150-186), p[3] "B does not come from the block's own B" (its code: 1 + p3, SAME_B 1, SAME_M 2),
+// p[4] and p[5] the K cell's code less 4, high and low bit (PREV_K 4, PREV_B 5, PREV_M 6).  All six come out of scalar logic on the
+// compares' result registers;
 // the priority of the equality chain ("the largest index whose candidate equals the maximum", r9.inl:138-143) is scalar logic:
 //   e4 -> 100, e3 & ~e4 -> 101, e2 & ~e3 & ~e4 -> 001, e1 & ~(e2 | e3 | e4) -> 110, none -> 010
 //   bit0 = (e3 | e2) & ~e4,   bit1 = ~(e4 | e3 | e2),   bit2 = e4 | e3 | (e1 & bit1);   soft (block 0 of row 1): all three set
@@ -143,15 +137,26 @@ __device__ __forceinline__ void ea_block_mb(float& M, float& B, const float lM_p
     const float newB = __builtin_fmaxf(b0, b2);
     const uint64_t pb = __builtin_amdgcn_ballot_w64(b2 >= b0);
     M = newM; B = newB;
-    p[0] = c0; p[1] = c1; p[2] = c2; p[3] = pb;
+    p[0] = c0; p[1] = c1; p[2] = c2; p[3] = ~pb;
 }
 __device__ __forceinline__ void ea_block_k(float& K, const float lM_r, const float lB_r, const float lK_r, const ea_trans& tr, uint64_t* __restrict__ p)
 {
     const float k1 = tr.mk + lM_r, k3 = tr.bk + lB_r, k4 = tr.kk + lK_r;
     const float newK = __builtin_fmaxf(__builtin_fmaxf(k1, k3), k4);
-    const uint64_t q4 = __builtin_amdgcn_ballot_w64(k4 == newK), q3 = __builtin_amdgcn_ballot_w64(k3 == newK) & ~q4;
+    const uint64_t q4 = __builtin_amdgcn_ballot_w64(k4 == newK), q3 = __builtin_amdgcn_ballot_w64(k3 == newK);
     K = newK;
-    p[4] = q4; p[5] = q3;
+    p[4] = ~(q3 | q4); p[5] = q3 & ~q4;
+}
+// x = 64 x + the lane's bits of the six masks of a block (M high to low, B, K high to low: see the line's layout above).  One add with
+// carry per mask.  (The compiler does not look for hazards inside the block: the masks are scalar logic's results, and should it ever
+// put a compare's own result here, the two idle states are what a vector read of it needs.)
+__device__ __forceinline__ uint32_t ea_pack(uint32_t x, const uint64_t* __restrict__ p)
+{
+    asm("s_nop 1\n\t"
+        "v_addc_co_u32_e64 %0, vcc, %0, %0, %1\n\tv_addc_co_u32_e64 %0, vcc, %0, %0, %2\n\tv_addc_co_u32_e64 %0, vcc, %0, %0, %3\n\t"
+        "v_addc_co_u32_e64 %0, vcc, %0, %0, %4\n\tv_addc_co_u32_e64 %0, vcc, %0, %0, %5\n\tv_addc_co_u32_e64 %0, vcc, %0, %0, %6"
+        : "+v"(x) : "s"(p[2]), "s"(p[1]), "s"(p[0]), "s"(p[3]), "s"(p[4]), "s"(p[5]) : "vcc");
+    return x;
 }
 
 struct ea_seg { const float* ev; int e_start, stride, e, n; };
@@ -163,7 +168,6 @@ template <int BPL>
 __device__ __attribute__((noinline)) float2 ea_fill2(const ea_gauss<BPL> G, const ea_trans tr, const float flank0, const ea_seg s0, const ea_seg s1,
                                                      uint8_t* __restrict__ bp, const int lane)
 {
-    constexpr int LINE = NP_EA2_LINE_BYTES(BPL);
     const int sl = lane & 31;
     const bool hi_half = lane >= 32;
     const int lu0 = (s0.n + BPL - 1) / BPL, lu1 = (s1.n + BPL - 1) / BPL;
@@ -187,7 +191,10 @@ __device__ __attribute__((noinline)) float2 ea_fill2(const ea_gauss<BPL> G, cons
     asm("" : "+v"(d0), "+v"(d1));                          // (vector registers: an addition with a scalar-register source issues in the slow class)
     float xn;                                             // the lane's event of the NEXT step
     { const float xa = buf_f32(evr0, off0), xb = buf_f32(evr1, off1); xn = hi_half ? xb : xa; }
-    const uint8_t* sline = ea_uniform(bp);                // (wave-uniform: the scalar stores' base)
+    // line t - 1: the wave's 64 dwords of step t (device memory by name: through a generic pointer the store would be a flat one, which
+    // makes every later wait for an event load a wait for the store too)
+    typedef __attribute__((address_space(1))) uint32_t global_u32;
+    global_u32* lines = (global_u32*)ea_uniform(bp);
     // the first lane of a half has no left neighbour (block -1 = -inf): instead of a select after the lane shift, the shift ADDS a
     // per-lane constant -- -inf in lanes 0 and 32, else 0 (v + 0 == v for every value the lattice holds, v + -inf == -inf) -- in the
     // same DPP instruction (bound_ctrl: lane 0's missing source reads as 0)
@@ -199,11 +206,6 @@ __device__ __attribute__((noinline)) float2 ea_fill2(const ea_gauss<BPL> G, cons
     };
     float soft = sl == 0 ? flank0 : NP_NEG_INF;                                  // HMT_FROM_SOFT: block 0 of row 1 only (flags 0)
     auto step = [&](const int t) {
-#ifndef NP_EA_NOWAIT
-        // the previous step's scalar stores have had a whole step to finish: their data registers are free again from here on
-        // (NP_EA_NOWAIT: timing experiment -- the wait costs nothing measurable)
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#endif
         const float nM = shr_add(M[BPL - 1]), nB = shr_add(B[BPL - 1]), nK = shr_add(K[BPL - 1]);
         const float x = xn;
         off0 += d0; off1 += d1;
@@ -217,19 +219,10 @@ __device__ __attribute__((noinline)) float2 ea_fill2(const ea_gauss<BPL> G, cons
         for (int c = 1; c < BPL; ++c) ea_block_k(K[c], M[c - 1], B[c - 1], K[c - 1], tr, pl + 6 * c);
         oM = nM; oB = nB; oK = nK;
         soft = NP_NEG_INF;
-        // ONE asm block issues the line's stores: every plane stays in its own scalar registers until all of them are on their way
-        const uint8_t* lp = sline + (size_t)(t - 1) * LINE;
-        asm volatile("s_store_dwordx2 %1, %0, 0x0\n\ts_store_dwordx2 %2, %0, 0x8\n\ts_store_dwordx2 %3, %0, 0x10\n\ts_store_dwordx2 %4, %0, 0x18\n\t"
-                     "s_store_dwordx2 %5, %0, 0x20\n\ts_store_dwordx2 %6, %0, 0x28\n\ts_store_dwordx2 %7, %0, 0x30\n\ts_store_dwordx2 %8, %0, 0x38\n\t"
-                     "s_store_dwordx2 %9, %0, 0x40\n\ts_store_dwordx2 %10, %0, 0x48\n\ts_store_dwordx2 %11, %0, 0x50\n\ts_store_dwordx2 %12, %0, 0x58\n\t"
-                     "s_store_dwordx2 %13, %0, 0x60\n\ts_store_dwordx2 %14, %0, 0x68\n\ts_store_dwordx2 %15, %0, 0x70\n\ts_store_dwordx2 %16, %0, 0x78\n\t"
-                     "s_store_dwordx2 %17, %0, 0x80\n\ts_store_dwordx2 %18, %0, 0x88"
-                     :: "s"(lp), "s"(pl[0]), "s"(pl[1]), "s"(pl[2]), "s"(pl[3]), "s"(pl[4]), "s"(pl[5]), "s"(pl[6]), "s"(pl[7]), "s"(pl[8]), "s"(pl[9]),
-                        "s"(pl[10]), "s"(pl[11]), "s"(pl[12]), "s"(pl[13]), "s"(pl[14]), "s"(pl[15]), "s"(pl[16]), "s"(pl[17]) : "memory");
-        if constexpr (BPL == 4)
-            asm volatile("s_store_dwordx2 %1, %0, 0x90\n\ts_store_dwordx2 %2, %0, 0x98\n\ts_store_dwordx2 %3, %0, 0xa0\n\ts_store_dwordx2 %4, %0, 0xa8\n\t"
-                         "s_store_dwordx2 %5, %0, 0xb0\n\ts_store_dwordx2 %6, %0, 0xb8"
-                         :: "s"(lp), "s"(pl[6 * BPL - 6]), "s"(pl[6 * BPL - 5]), "s"(pl[6 * BPL - 4]), "s"(pl[6 * BPL - 3]), "s"(pl[6 * BPL - 2]), "s"(pl[6 * BPL - 1]) : "memory");
+        uint32_t word = 0u;
+#pragma unroll
+        for (int c = BPL - 1; c >= 0; --c) word = ea_pack(word, pl + 6 * c);
+        lines[(size_t)(t - 1) * (NP_EA2_LINE_BYTES / 4) + lane] = word;
     };
     int t = 1;
     for (; t + 1 <= s_min; t += 2) { step(t); step(t + 1); }      // two steps per iteration: the values a step hands to the next need no move back to fixed registers
@@ -241,8 +234,6 @@ __device__ __attribute__((noinline)) float2 ea_fill2(const ea_gauss<BPL> G, cons
     for (int c = 0; c < BPL; ++c) zM[c] = M[c];
     for (; t + 1 <= s_max; t += 2) { step(t); step(t + 1); }
     for (; t <= s_max; ++t) step(t);
-    // the lines sit in the scalar data cache: write them back to L2, where the walk's loads (at agent scope: past the vector L1) find them
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb\n\ts_waitcnt lgkmcnt(0)" ::: "memory");
     const int ec_0 = s0.n > 0 ? (s0.n - 1) % BPL : 0, ec_1 = s1.n > 0 ? (s1.n - 1) % BPL : 0;
     const int my_ec = hi_half ? ec_1 : ec_0;
     float live = M[0], snap = zM[0];
@@ -349,51 +340,42 @@ __device__ __attribute__((noinline)) void ea_next_segment(const np_ea_args* __re
 // 32..63 half 1's (every lane of a half computes the same).  A walk step is one dependent chain around an LDS read; as scalar
 // code, one segment after the other, it took ~550-790 cycles per step and half of this kernel's time (the scalar unit's latency
 // per dependent instruction, ~40-55 of them per step), and two scalar chains interleaved in one loop were no faster.  As vector
-// code the chain is ~25 instructions for BOTH segments, and the back-pointer word is already the move (ea_block).
-// Per half: a window of WIN lines of its planes staged in LDS (refilled when the walk leaves it) and the list of visited
+// code the chain is ~25 instructions for BOTH segments.
+// Per half: a window of NP_EA_WIN lines of its dwords staged in LDS (refilled when the walk leaves it) and the list of visited
 // states in LDS (ea_lds; a longer path spills the full buffer to the half's global list and goes on).
 typedef __attribute__((address_space(3))) uint32_t lds_u32;
 #ifndef NP_EA_EARLY
 #define NP_EA_EARLY 5                     // refill a window that has fewer than this many lines left (experiment)
 #endif
-#define NP_EA_STAGE 568                   // dwords of a half's window
+#define NP_EA_WIN 24                      // lines of a half's window: three rounds of 64 lanes' 16-byte requests
+#define NP_EA_LDW 32                      // dwords of a half's line
 #ifndef NP_EA_BCAP
-#define NP_EA_BCAP 176                    // bursts of a half's list that LDS holds (a longer list spills to the half's global list)
+#define NP_EA_BCAP 112                    // bursts of a half's list that LDS holds (a longer list spills to the half's global list): twenty
+                                          // waves' blocks fit a CU's LDS beside their windows
 #endif
 #define NP_EA_BURST 10                    // steps of a burst at most: their codes share a dword
 // The list of visited states, per half: one 64-bit word per BURST of walk steps (round 5; until then one dword per visited state, written
 // by every step -- six of a step's vector instructions).  Low dword: the state the burst starts in, row | k-mer << 16 | state << 24, and
 // the number of steps << 26; high dword: the steps' move codes, three bits each, first step lowest.  The emission replays a burst from
 // its first state (row -= state != KMER_SKIP, k-mer -= code >> 2, state = code & 3).
-struct ea_lds {
-    uint32_t stage[2][NP_EA_STAGE];        // back-pointer windows
+struct alignas(16) ea_lds {
+    uint32_t stage[2][NP_EA_WIN * NP_EA_LDW];        // back-pointer windows
     uint64_t bursts[2][NP_EA_BCAP];        // oldest first
     ea_wave_state W;
 };
+static_assert(20 * sizeof(ea_lds) <= 163840, "twenty waves of a CU");
 typedef __attribute__((address_space(3))) uint64_t lds_u64;
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 struct ea_walk_result { int nb0, nb1, spilled0, spilled1; };       // bursts in all, bursts spilled
 
-// The window in LDS holds a block's back-pointers as NINE dwords, three per state: the state's move code bit by bit, so that a walk
-// step reads the three dwords of the state it is in and needs no arithmetic on them (round 5; until then the six planes as the sweep
-// stores them, every step decoding all three states' codes and selecting one: 14 of its 41 vector instructions):
-//   +0..2  KMER_SKIP (state 0):  q3, ~(q3 | q4), ~0   (code 6 - q3 - 2 q4: PREV_K 4 / PREV_B 5 / PREV_M 6)
-//   +3..5  BAD_EVENT (state 1):  pb, ~pb, 0           (code 2 - pb: SAME_B 1 / SAME_M 2)
-//   +6..8  MATCH (state 2):      the three planes of the M cell's code as stored
-// The refill makes the complements; the two constant dwords of every cell are written once per launch (ea_window_init).
-#define NP_EA_CELL 9
-__host__ __device__ constexpr int ea_window_lines(int bpl)
-{
-    // as many lines as three rounds of 64 lanes' 16-byte requests bring in, and as the half's stage holds
-    return (192 / (3 * bpl)) < (NP_EA_STAGE / (NP_EA_CELL * bpl)) ? (192 / (3 * bpl)) : (NP_EA_STAGE / (NP_EA_CELL * bpl));
-}
-template <int BPL> __device__ __forceinline__ void ea_window_init(ea_lds* L, const int lane)
-{
-    for (int i = lane; i < 2 * ea_window_lines(BPL) * BPL; i += 64) {
-        const int h = i / (ea_window_lines(BPL) * BPL), cell = i - h * ea_window_lines(BPL) * BPL;
-        L->stage[h][cell * NP_EA_CELL + 2] = ~0u; L->stage[h][cell * NP_EA_CELL + 5] = 0u;
-    }
-}
+// A walk step takes its move from the dword of the lane that owns the k-mer: bits pos .. pos + width - 1 of it plus a bias, by the state
+// walked in (0 KMER_SKIP, 1 BAD_EVENT, 2 MATCH); pos = 6 (k % BPL) + the state's first bit.  The three numbers of a state are bytes of
+// constants.
+#define NP_EA_FIRST 0x030200u
+#define NP_EA_WIDTH 0x030102u
+#define NP_EA_BIAS  0x000104u
 
 // the lane (of its half) that owns k-mer k = k / BPL, as full-rate instructions (a 32-bit multiply-high is quarter rate); 5 bits, as the
 // shifts that use it take
@@ -415,8 +397,7 @@ template <int BPL>
 __device__ __attribute__((noinline)) ea_walk_result ea_walk2(ea_lds* L, const float sv0_, const float sv1_, const uint8_t* __restrict__ bp_,
                                                              uint32_t* __restrict__ path0_, uint32_t* __restrict__ path1_, const int lane)
 {
-    constexpr int LINE = NP_EA2_LINE_BYTES(BPL), PER_LINE = 3 * BPL;      // PER_LINE: 16-byte pieces (two planes) of a line
-    constexpr int CELL = NP_EA_CELL, LSTR = CELL * BPL, WIN = ea_window_lines(BPL);
+    constexpr int LINE = NP_EA2_LINE_BYTES, WIN = NP_EA_WIN;
     const float sv0 = ea_uniform(sv0_), sv1 = ea_uniform(sv1_);
     const uint8_t* __restrict__ bp = ea_uniform(bp_);
 
@@ -432,22 +413,10 @@ __device__ __attribute__((noinline)) ea_walk_result ea_walk2(ea_lds* L, const fl
     bool alive = (hi_half ? (H1.ri >= 0 && sv1 != NP_NEG_INF) : (H0.ri >= 0 && sv0 != NP_NEG_INF)) && e > 0 && n > 0;
     // (L arrives as a generic pointer -- a not-inlined function's argument; without the address space the compiler reads the staged
     //  lines with flat loads behind null checks and 64-bit address arithmetic, in the middle of the walk's dependent chain)
-    const lds_u32* st = (const lds_u32*)&L->stage[hi_half ? 1 : 0][0];
+    const lds_u8* st = (const lds_u8*)&L->stage[hi_half ? 1 : 0][0];
     lds_u64* bl = (lds_u64*)&L->bursts[hi_half ? 1 : 0][0];
-    // what this lane does in a refill, whatever the window: piece i = lane + 64 it is 16-byte piece q (planes 2q, 2q + 1) of line ln; of a
-    // block's six planes, pieces 0 / 1 / 2 hold (M0, M1) / (M2, pb) / (q4, q3).  The lane writes two values to g_a, g_a + 1 -- (M0, M1) /
-    // (pb, ~pb) / (q3, ~(q3 | q4)) -- and a third to g_b: piece 1 its M2, the others their second value once more (no dump slot)
-    int g_off[3]; uint32_t g_a[3], g_b[3]; bool g_first[3], g_k[3], g_p[3];
-#pragma unroll
-    for (int it = 0; it < 3; ++it) {
-        const int i = lane + 64 * it, ln = i / PER_LINE, q = i - PER_LINE * ln, c = q / 3, part = q - 3 * c;
-        g_off[it] = ln * LINE + q * 16;
-        g_a[it] = (uint32_t)((ln * BPL + c) * CELL + (part == 0 ? 6 : part == 1 ? 3 : 0));
-        g_b[it] = part == 1 ? g_a[it] + 5u : g_a[it] + 1u;
-        g_first[it] = part == 0; g_k[it] = part == 2; g_p[it] = part == 1;
-    }
-    const bool g_live2 = (lane + 128) / PER_LINE < WIN;      // the third round's pieces past the window's last line
-    static_assert(127 / PER_LINE < WIN, "the first two rounds' pieces are inside the window");
+    static_assert(WIN * NP_EA_LDW * 4 % (64 * 16) == 0, "whole rounds of 16-byte requests");
+    constexpr int ROUNDS = WIN * NP_EA_LDW * 4 / (64 * 16);
     while (__builtin_amdgcn_ballot_w64(alive) != 0ull) {
         // ---- per half, by scalar control: refill the window of a walk that is outside it; spill a full list ----
         const int line0 = (int)((uint32_t)row + (uint32_t)k / BPL);
@@ -459,21 +428,18 @@ __device__ __attribute__((noinline)) ea_walk_result ea_walk2(ea_lds* L, const fl
             if ((need_m >> (32 * h)) & 1ull) {
                 const int hi = __builtin_amdgcn_readlane(line0, 32 * h);
                 const int nlo = hi - (WIN - 1) > 1 ? hi - (WIN - 1) : 1;
-                // dword h of every plane of every line of the window, PER_LINE 16-byte requests per line (two planes each), all of a refill in
-                // flight at once, at agent scope: they bypass the vector L1, which may still hold the previous segment's lines at these
-                // addresses (the sweep wrote the new ones through the scalar cache).  A piece past the window's last line is outside the
-                // descriptor's range and reads as 0 (what it writes, nobody reads).
+                // the half's 128 bytes of every line of the window, eight 16-byte requests per line (lane i of round r: piece i & 7 of line
+                // 8 r + i / 8), all of a refill in flight at once, at agent scope: they bypass the vector L1, which may still hold the
+                // previous segment's lines at these addresses.  A piece past the window's last line is outside the descriptor's range and
+                // reads as 0 (nobody reads it).
                 const __amdgpu_buffer_rsrc_t lr = make_rsrc(bp + (size_t)(nlo - 1) * LINE, (uint32_t)(hi - nlo + 1) * LINE);
-                lds_u32* dst = (lds_u32*)&L->stage[h][0];
-                uint4 v[3];
+                u32x4 v[ROUNDS];
 #pragma unroll
-                for (int it = 0; it < 3; ++it) v[it] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(lr, whole_offset(g_off[it]), 0, 16 /* sc1 */));
+                for (int it = 0; it < ROUNDS; ++it)
+                    v[it] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(lr, whole_offset((8 * it + (lane >> 3)) * LINE + h * (LINE / 2) + (lane & 7) * 16), 0, 16 /* sc1 */));
+                lds_u32x4* dst = (lds_u32x4*)&L->stage[h][0];
 #pragma unroll
-                for (int it = 0; it < 3; ++it) {
-                    const uint32_t pa = h ? v[it].y : v[it].x, pb2 = h ? v[it].w : v[it].z;
-                    const uint32_t w0 = g_first[it] ? pa : pb2, w1 = g_first[it] ? pb2 : ~(pb2 | (g_k[it] ? pa : 0u)), w2 = g_p[it] ? pa : w1;
-                    if (it < 2 || g_live2) { dst[g_a[it]] = w0; dst[g_a[it] + 1] = w1; dst[g_b[it]] = w2; }
-                }
+                for (int it = 0; it < ROUNDS; ++it) dst[64 * it + lane] = v[it];
                 lo = (hi_half == (h == 1)) ? nlo : lo;
             }
             if ((full_m >> (32 * h)) & 1ull) {
@@ -493,23 +459,23 @@ __device__ __attribute__((noinline)) ea_walk_result ea_walk2(ea_lds* L, const fl
         const int mine = alive ? room : NP_EA_BURST;
         const int b0 = __builtin_amdgcn_readlane(mine, 0), b1 = __builtin_amdgcn_readlane(mine, 32);
         const int b01 = b0 < b1 ? b0 : b1, burst = b01 < NP_EA_BURST ? b01 : NP_EA_BURST;
-        // codes of cell (row, k): stage[(row + k / BPL - lo) * LSTR + (k % BPL) * CELL ...] = stage[CELL * (row * BPL + k - lo * BPL) ...]: an
-        // offset that falls by CELL * BPL with the row and by CELL with the k-mer.  (A finished walk's offset is anything: the min keeps
-        // its reads inside the window.)
-        uint32_t off = ((uint32_t)row * BPL + (uint32_t)k - (uint32_t)lo * BPL) * (CELL * 4u);      // (in bytes)
+        // the dword of cell (row, k): stage[(row + k / BPL - lo) * 32 + k / BPL], i.e. byte 128 (row - lo) + 132 (k / BPL).  (A finished
+        // walk's offset is anything: the min keeps its reads inside the window.)
+        const uint32_t lo128 = (uint32_t)lo * (4u * NP_EA_LDW);
         const uint32_t first = (uint32_t)row | ((uint32_t)k << 16) | ((uint32_t)ps << 24);
         uint32_t codes = 0u;
         uint32_t steps0 = 0u, steps1 = 0u;                // steps each half's walk was alive at
         uint64_t am = __builtin_amdgcn_ballot_w64(alive); // inside the burst "alive" is this scalar mask, the counts scalar additions
         for (int s = 0; s < burst; ++s) {
             steps0 += (uint32_t)am & 1u; steps1 += (uint32_t)(am >> 32) & 1u;
-            // the move out of this cell: the three dwords of the state walked in, of each the bit of the lane that owns the k-mer
-            const lds_u32* pw = (const lds_u32*)((const lds_u8*)st + ((off < (uint32_t)((WIN * BPL - 1) * CELL * 4) ? off : (uint32_t)((WIN * BPL - 1) * CELL * 4)) + ea_mul24((uint32_t)ps, 12u)));
-            const uint32_t w0 = pw[0], w1 = pw[1], w2 = pw[2];
-            const uint32_t k3 = ea_owner<BPL>((uint32_t)k);
-            const uint32_t c = __builtin_amdgcn_ubfe(w0, k3, 1) | (__builtin_amdgcn_ubfe(w1, k3, 1) << 1) | (__builtin_amdgcn_ubfe(w2, k3, 1) << 2);
+            // the move out of this cell: the dword of the lane that owns the k-mer, of it the state's field of the k-mer's block
+            const uint32_t own = ea_owner<BPL>((uint32_t)k);
+            const uint32_t off = ea_mul24(own, 4u * NP_EA_LDW + 4u) + (((uint32_t)row * (4u * NP_EA_LDW)) - lo128);
+            const uint32_t w = *(const lds_u32*)(st + (off < (uint32_t)(4 * (WIN * NP_EA_LDW - 1)) ? off : (uint32_t)(4 * (WIN * NP_EA_LDW - 1))));
+            const uint32_t b8 = (uint32_t)ps * 8u;
+            const uint32_t pos = ea_mul24((uint32_t)k - ea_mul24(own, BPL), 6u) + __builtin_amdgcn_ubfe(NP_EA_FIRST, b8, 8);
+            const uint32_t c = __builtin_amdgcn_ubfe(w, pos, __builtin_amdgcn_ubfe(NP_EA_WIDTH, b8, 8)) + __builtin_amdgcn_ubfe(NP_EA_BIAS, b8, 8);
             codes |= c << (3 * s);
-            off -= ((c & 4u) != 0u ? (uint32_t)(CELL * 4) : 0u) + (ps != 0 ? (uint32_t)(LSTR * 4) : 0u);
             row -= ps != 0 ? 1 : 0;                                     // K states are silent (r9.cpp:176-178)
             k -= (int)(c >> 2);
             ps = (int)(c & 3u);
@@ -621,7 +587,6 @@ __global__ void __launch_bounds__(64, WAVES) np_eventalign_chain2_kernel(const n
     uint32_t* __restrict__ path = a.path + (size_t)wave_slot * a.path_stride;
     const int k = a.k;
     if (lane == 0) { W.h[0].ri = -1; W.h[1].ri = -1; W.drained = 0; }
-    ea_window_init<BPL>(&lds, lane);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     __builtin_amdgcn_s_waitcnt(0);
     __builtin_amdgcn_wave_barrier();
@@ -705,5 +670,5 @@ hipError_t np_launch_eventalign_chain(const np_ea_args& a, const np_ea_args* a_d
     else hipLaunchKernelGGL((np_eventalign_chain2_kernel<4, 4>), dim3(n_blocks), dim3(64), 0, s, a_dev);
     return hipGetLastError();
 }
-int np_eventalign_line_bytes(int variant) { return variant == 4 ? NP_EA2_LINE_BYTES(4) : NP_EA2_LINE_BYTES(3); }
+int np_eventalign_line_bytes(int variant) { (void)variant; return NP_EA2_LINE_BYTES; }
 int np_eventalign_max_kmers(int variant) { return variant == 4 ? 128 : 96; }

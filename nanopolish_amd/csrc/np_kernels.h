@@ -46,7 +46,7 @@ struct np_ea_args {
     const int32_t* read_len;
     const uint8_t* read_rc;
     int k;
-    uint8_t* bp;                   // per-wave back-pointer scratch: rows_cap x 128 B
+    uint8_t* bp;                   // per-wave back-pointer scratch: a 256-byte line per sweep step
     size_t bp_stride;
     int rows_cap;
     int max_kmers;                 // k-mers per segment the launched instantiation holds (32 lanes x blocks per lane)
