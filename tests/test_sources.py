@@ -4,7 +4,7 @@ import os
 import re
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-DIRS = ["nanopolish_amd/csrc"]
+DIRS = ["nanopolish_amd/csrc", "tools"]
 
 
 def _gpu_sources():

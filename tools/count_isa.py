@@ -30,7 +30,7 @@ def klass(op):
     if op.startswith("v_"): return "valu"
     if op.startswith(("s_waitcnt", "s_nop", "s_setprio")): return "wait"
     if op.startswith(("s_cbranch", "s_branch")): return "branch"
-    if op.startswith(("s_load", "s_store", "s_buffer")): return "smem"
+    if op.startswith(("s_load", "s_buffer")): return "smem"
     if op.startswith("s_"): return "salu"
     if op.startswith(("buffer_", "global_", "flat_", "scratch_")): return "vmem"
     if op.startswith("ds_"): return "lds"

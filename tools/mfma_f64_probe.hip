@@ -39,18 +39,15 @@ __global__ void k_add(double* o_m, double* o_v, const double* ident, const doubl
     }
 }
 
-// MODE 6: as 0, but the four compare masks are stored by two s_store_dwordx4 instead of four v_addc (trace as lane-mask planes)
 // MODE 0: ten v_add_f64 + the rest of a band on the vector port; 1: the ten additions as MFMAs; 2: no additions; 3: MFMAs only;
 // 4: the vector rest only counted as in 2 but with ten s_nop (issue slots without a pipe); 5: ten v_add_f64 only
 #define REP10(X) X(0) X(1) X(2) X(3) X(4) X(5) X(6) X(7) X(8) X(9)
 #define TRACE_ADDC "v_addc_co_u32_e64 %[t], s[28:29], %[t], %[t], s[20:21]\n v_addc_co_u32_e64 %[t], s[28:29], %[t], %[t], s[22:23]\n" \
                    "v_addc_co_u32_e64 %[t], s[28:29], %[t], %[t], s[24:25]\n v_addc_co_u32_e64 %[t], s[28:29], %[t], %[t], s[26:27]\n"
-// the four compare masks leave through the scalar data cache instead (two 16-byte scalar stores per band)
 #define TRACE_FLOAT "v_sub_f32 %[x0], %[a6], %[a0]\n v_sub_f32 %[x1], %[a6], %[a1]\n v_sub_f32 %[x2], %[a7], %[a2]\n v_sub_f32 %[x3], %[a7], %[a3]\n" \
                     "v_fma_f32 %[x0], %[x0], %[big], %[one] clamp\n v_fma_f32 %[x1], %[x1], %[big], %[one] clamp\n v_fma_f32 %[x2], %[x2], %[big], %[one] clamp\n v_fma_f32 %[x3], %[x3], %[big], %[one] clamp\n" \
                     "v_fma_f32 %[x0], %[x0], %[two], %[x1]\n v_fma_f32 %[x2], %[x2], %[two], %[x3]\n v_fma_f32 %[f0], %[f0], %[four], %[x0]\n v_fma_f32 %[f1], %[f1], %[four], %[x2]\n"
-#define TRACE_SSTORE "s_store_dwordx4 s[20:23], %[sp], 0x0\n s_store_dwordx4 s[24:27], %[sp], 0x10\n"
-template <int MODE> __global__ void __launch_bounds__(256, 8) k_mix(unsigned long long* out, double* sink, const double* ident, int iters, uint64_t* splane = nullptr)
+template <int MODE> __global__ void __launch_bounds__(256, 8) k_mix(unsigned long long* out, double* sink, const double* ident, int iters)
 {
     const int l = threadIdx.x & 63;
     const double A = ident[l];
@@ -65,34 +62,13 @@ template <int MODE> __global__ void __launch_bounds__(256, 8) k_mix(unsigned lon
     for (int i = 0; i < iters; ++i) {
 #define VADD(n) asm volatile("v_add_f64 %0, %0, %1" : "+v"(d##n) : "v"(B));
 #define MADD(n) d##n = __builtin_amdgcn_mfma_f64_4x4x4f64(A, B, d##n, 0, 0, 0);
-        if (MODE == 0 || MODE == 5 || MODE == 6 || MODE == 8 || MODE == 9) { REP10(VADD) }
+        if (MODE == 0 || MODE == 5 || MODE == 8 || MODE == 9) { REP10(VADD) }
         if (MODE == 1 || MODE == 3) { REP10(MADD) }
         if (MODE == 4) { asm volatile("s_nop 0\n s_nop 0\n s_nop 0\n s_nop 0\n s_nop 0\n s_nop 0\n s_nop 0\n s_nop 0\n s_nop 0\n s_nop 0"); }
         if (MODE != 3 && MODE != 5) {
             // the band's other 44 vector instructions by class: 18 fast fp32, 5 + 6 conversions, 4 compares to scalar pairs + 4 carry adds,
             // 2 max3, 2 selects, 1 DPP rotate, 2 lane reads
-            if (MODE == 6 || MODE == 7) {
-                const uint64_t* sp = splane + ((size_t)(blockIdx.x * 4 + (threadIdx.x >> 6)) * 4096 + (size_t)(i & 1023) * 4);      // 32 B per band, a 32 KB window per wave
-                sp = (const uint64_t*)(((uint64_t)__builtin_amdgcn_readfirstlane((int)((uint64_t)sp >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint64_t)sp));
-            asm volatile(
-                "v_fma_f32 %[a0], %[a0], %[a1], %[a2]\n v_fma_f32 %[a1], %[a1], %[a2], %[a3]\n v_fma_f32 %[a2], %[a2], %[a3], %[a4]\n"
-                "v_fma_f32 %[a3], %[a3], %[a4], %[a5]\n v_fma_f32 %[a4], %[a4], %[a5], %[a6]\n v_fma_f32 %[a5], %[a5], %[a6], %[a7]\n"
-                "v_mul_f32 %[a6], %[a6], %[a7]\n v_mul_f32 %[a7], %[a7], %[a0]\n v_sub_f32 %[a0], %[a0], %[a1]\n"
-                "v_fma_f32 %[a0], %[a0], %[a1], %[a2]\n v_fma_f32 %[a1], %[a1], %[a2], %[a3]\n v_fma_f32 %[a2], %[a2], %[a3], %[a4]\n"
-                "v_fma_f32 %[a3], %[a3], %[a4], %[a5]\n v_fma_f32 %[a4], %[a4], %[a5], %[a6]\n v_fma_f32 %[a5], %[a5], %[a6], %[a7]\n"
-                "v_mul_f32 %[a6], %[a6], %[a7]\n v_mul_f32 %[a7], %[a7], %[a0]\n v_sub_f32 %[a0], %[a0], %[a1]\n"
-                "v_cvt_f64_f32 %[e0], %[a0]\n v_cvt_f64_f32 %[e1], %[a1]\n v_cvt_f64_f32 %[e2], %[a2]\n v_cvt_f64_f32 %[e3], %[a3]\n v_cvt_f64_f32 %[e4], %[a4]\n"
-                "v_cvt_f32_f64 %[a0], %[e0]\n v_cvt_f32_f64 %[a1], %[e1]\n v_cvt_f32_f64 %[a2], %[e2]\n v_cvt_f32_f64 %[a3], %[e3]\n v_cvt_f32_f64 %[a4], %[e4]\n v_cvt_f32_f64 %[a5], %[e0]\n"
-                "v_cmp_eq_f32_e64 s[20:21], %[a0], %[a1]\n v_cmp_eq_f32_e64 s[22:23], %[a1], %[a2]\n v_cmp_eq_f32_e64 s[24:25], %[a2], %[a3]\n v_cmp_eq_f32_e64 s[26:27], %[a3], %[a4]\n"
-                TRACE_SSTORE
-                "v_max3_f32 %[a6], %[a6], %[a0], %[a1]\n v_max3_f32 %[a7], %[a7], %[a2], %[a3]\n"
-                "v_cndmask_b32_e64 %[a6], %[a6], %[a4], s[20:21]\n v_cndmask_b32_e64 %[a7], %[a7], %[a5], s[22:23]\n"
-                "v_mov_b32_dpp %[a5], %[a7] wave_ror:1 row_mask:0xf bank_mask:0xf\n"
-                "v_readlane_b32 s30, %[a6], 5\n v_readlane_b32 s31, %[a7], 9\n"
-                : [a0] "+v"(a0), [a1] "+v"(a1), [a2] "+v"(a2), [a3] "+v"(a3), [a4] "+v"(a4), [a5] "+v"(a5), [a6] "+v"(a6), [a7] "+v"(a7),
-                  [e0] "+v"(e0), [e1] "+v"(e1), [e2] "+v"(e2), [e3] "+v"(e3), [e4] "+v"(e4), [t] "+v"(t)
-                : [sp] "s"(sp) : "memory", "s20", "s21", "s22", "s23", "s24", "s25", "s26", "s27", "s28", "s29", "s30", "s31");
-            } else if (MODE == 8 || MODE == 9) {
+            if (MODE == 8 || MODE == 9) {
             // MODE 8 (round 6, late): the trace WITHOUT compares and carry adds -- per candidate a float difference, a clamped fma that turns
             // "difference == 0" into 1.0 / 0.0, and per cell two fmas that shift the two bits into a float accumulator: 12 fast-class
             // instructions for the 8 slow ones.  MODE 9: no trace instructions at all (the bound).
@@ -142,7 +118,6 @@ template <int MODE> __global__ void __launch_bounds__(256, 8) k_mix(unsigned lon
 
         }
     }
-    if (MODE == 6 || MODE == 7) asm volatile("s_dcache_wb\n s_waitcnt lgkmcnt(0)" ::: "memory");
     const unsigned long long c1 = __builtin_readcyclecounter();
     const unsigned long long t1 = wall_clock64();
     if (threadIdx.x == 0) { out[2 * blockIdx.x] = c1 - c0; out[2 * blockIdx.x + 1] = t1 - t0; }
@@ -279,14 +254,13 @@ template <int MODE> static int run_mix(const char* name, const double* ident_d, 
     const int cus = p.multiProcessorCount;
     const int blocks = cus * waves_per_simd;          // 256-thread blocks: 4 waves, one per SIMD
     const int iters = 20000;
-    unsigned long long* out; double* sink; uint64_t* splane = nullptr;
+    unsigned long long* out; double* sink;
     CK(hipMalloc(&out, blocks * 16)); CK(hipMalloc(&sink, (size_t)blocks * 256 * 8));
-    if (MODE == 6 || MODE == 7) CK(hipMalloc(&splane, (size_t)blocks * 4 * 4096 * 8));
     hipEvent_t e0, e1; CK(hipEventCreate(&e0)); CK(hipEventCreate(&e1));
-    hipLaunchKernelGGL(k_mix<MODE>, dim3(blocks), dim3(256), 0, 0, out, sink, ident_d, 200, splane);
+    hipLaunchKernelGGL(k_mix<MODE>, dim3(blocks), dim3(256), 0, 0, out, sink, ident_d, 200);
     CK(hipDeviceSynchronize());
     CK(hipEventRecord(e0));
-    hipLaunchKernelGGL(k_mix<MODE>, dim3(blocks), dim3(256), 0, 0, out, sink, ident_d, iters, splane);
+    hipLaunchKernelGGL(k_mix<MODE>, dim3(blocks), dim3(256), 0, 0, out, sink, ident_d, iters);
     CK(hipEventRecord(e1)); CK(hipDeviceSynchronize());
     float ms; CK(hipEventElapsedTime(&ms, e0, e1));
     std::vector<unsigned long long> h(blocks * 2); CK(hipMemcpy(h.data(), out, blocks * 16, hipMemcpyDeviceToHost));
@@ -296,7 +270,7 @@ template <int MODE> static int run_mix(const char* name, const double* ident_d, 
     const double ns_per_iter_simd = ms * 1e6 / ((double)iters * waves_per_simd);
     printf("  %-34s waves/SIMD %d: %8.2f ms  %7.1f ns per iteration and SIMD-wave (= %6.1f cycles at 2.4 GHz)  s_memtime/iter %.1f  wall_clock/iter %.2f\n",
            name, waves_per_simd, ms, ns_per_iter_simd, ns_per_iter_simd * 2.4, cyc / iters, wc / iters);
-    CK(hipFree(out)); CK(hipFree(sink)); if (splane) CK(hipFree(splane));
+    CK(hipFree(out)); CK(hipFree(sink));
     return 0;
 }
 
@@ -384,7 +358,6 @@ int main()
         if (run_mix<8>("band, trace as 12 fast fp32 ops", ident_d, w)) return 1;
         if (run_mix<9>("band, no trace at all", ident_d, w)) return 1;
         if (run_mix<0>("band rest + 10 v_add_f64 (again)", ident_d, w)) return 1;
-        if (run_mix<6>("band (adds) - 4 addc + 2 s_store_x4", ident_d, w)) return 1;
     }
     printf("ring layouts (instruction-stream mock of the FAST band loop, no walk, no loads):\n");
     if (run_ring<2, 1, 2, 8>("2 slots/lane, 1 read/wave (shipped)", 1)) return 1;
