@@ -10,7 +10,7 @@
 //     "last aligned pair with ref_pos <= x" search), closest events from the read's event map (np_device.h);
 //   * Viterbi fill as an anti-diagonal sweep, two segments (of two reads) per wave, one per half-wave: lane j of a half owns three
 //     k-mer blocks (a segment has <= 96 k-mers; four for the k = 5 model), computes row t - j at step t; previous row in registers,
-//     left neighbour through DPP; candidates in HMMMovementType order, later index wins ties; only back-pointers leave the wave, six
+//     left neighbour through DPP; candidates in HMMMovementType order, later index wins ties; only back-pointers leave the wave, seven
 //     bits per block, one dword per lane and one 256-byte line per sweep STEP (cell (row r, k-mer b) sits in line r + b / BPL, dword
 //     b / BPL of its half), into a per-wave scratch (ea_fill2);
 //   * back-track of both halves' segments as vector code over a window of lines staged in LDS, in bursts of steps whose number is known in advance; the visited states go to a per-half list, one 64-bit word per burst
@@ -45,21 +45,19 @@ struct ea_trans { float mm_self, mb, mk, mm_next, bb, bk, bm_next, bm_self, kk, 
 // segment.  The per-read state that survives from segment to segment is ten integers per half (ea_half); what only depends on
 // the read's index is reloaded where it is needed (wave-uniform loads).
 // ---------------------------------------------------------------------------------------------------------------------------
-// Back-pointers: SIX bits per k-mer block.  The compares' results are lane masks in scalar registers; scalar logic, which has an issue
-// port of its own, turns them into six masks per block, and the lane's word takes one bit of each by an add with carry
-// (x = 2 x + mask bit: one vector instruction per mask):
-//   bits 5..3  the M cell's move code (3 bits)
-//   bit  2     the B cell's: code 1 + bit
-//   bits 1..0  the K cell's: code 4 + bits
-// block c of the lane in bits 6 c .. 6 c + 5 of its dword.  A line is 64 dwords, 256 bytes, one coalesced vector store: half h's walk
-// reads its 128-byte half of a line.
+// Back-pointers: SEVEN bits per k-mer block, "this candidate is the cell's maximum" for every candidate but each state's first (which is
+// the move when no other bit is set; of several set bits the reference's "later index wins" takes the highest candidate).  A bit is the
+// sign of (candidate - maximum), shifted into the lane's word: one subtraction and one v_alignbit_b32 per candidate, no lane masks.
+//   bits 5 c .. 5 c + 4              block c:  B from its own B;  M from K, B, own B, M to the left (PREV_K, PREV_B, SAME_B, PREV_M)
+//   bits 5 BPL + 2 (BPL - 1 - c) ..  block c:  K from PREV_K, PREV_B
+// i.e. in every state the bits rise as the candidates' indices fall, and the walk takes the lowest set one.  A line is 64 dwords, 256
+// bytes, one coalesced vector store: half h's walk reads its 128-byte half of a line.
+// Measured, 50 000 reads from raw signal: 229 ms; with lane masks (a compare per candidate) combined to six bits by scalar logic and added
+// into the word with carries 242 ms.
 // BPL, the k-mer blocks per lane: a segment spans up to 101 reference bases (eventalign.cpp:695-735), i.e. 102 - k k-mers: 96 for the
 // DNA models (k = 6: three blocks on each of a half-wave's 32 lanes), 97 for the direct-RNA model (k = 5): that one k-mer more takes a
-// fourth block per lane (np_eventalign_chain2_kernel<WAVES, 4>: the same code, 24 bits of the dword).
+// fourth block per lane (np_eventalign_chain2_kernel<WAVES, 4>: the same code, 28 bits of the dword).
 #define NP_EA2_LINE_BYTES 256
-#ifndef NP_EA_ARGMAX
-#define NP_EA_ARGMAX 1           // the M cell's arg-max: 0 = tournament (round 3), 1 = three-input maxima + equality chain (round 4)
-#endif
 
 // Arguments of a (not inlined) device function arrive in vector registers, and the compiler cannot know that they are wave-uniform:
 // everything computed from them would become vector code (the back-track as exec-masked vector loops, the argument block read with
@@ -106,57 +104,36 @@ struct ea_half {                 // chain state of the read a half-wave works on
 };
 
 // One k-mer block of one lattice row (the candidates of r9.inl:130-197 in HMMMovementType order, later index wins ties; (lM_r, lB_r,
-// lK_r): the block to the left in this row, (lM_p, ...): in the previous row) with the back-pointers as lane masks: p[0..2] the M cell's move code bit by bit (HMT_FROM_SAME_M 2, PREV_M 6,
-// SAME_B 1, PREV_B 5, PREV_K 4, SOFT 7: bit 2 = "the k-mer steps back", bits 1..0 = the state walked to, 2 MATCH, 1 BAD_EVENT, 0
-// KMER_SKIP; 7 = soft clip, stop -- r9.cpp:150-186), p[3] "B does not come from the block's own B" (its code: 1 + p3, SAME_B 1, SAME_M 2),
-// p[4] and p[5] the K cell's code less 4, high and low bit (PREV_K 4, PREV_B 5, PREV_M 6).  All six come out of scalar logic on the
-// compares' result registers;
-// the priority of the equality chain ("the largest index whose candidate equals the maximum", r9.inl:138-143) is scalar logic:
-//   e4 -> 100, e3 & ~e4 -> 101, e2 & ~e3 & ~e4 -> 001, e1 & ~(e2 | e3 | e4) -> 110, none -> 010
-//   bit0 = (e3 | e2) & ~e4,   bit1 = ~(e4 | e3 | e2),   bit2 = e4 | e3 | (e1 & bit1);   soft (block 0 of row 1): all three set
-// Round 4, second pass: the block in two halves so that a step needs no copy of the previous row.  The M and B cells of row r read row
-// r-1 of their own block and of the block to the left; K reads row r of the block to the left.  Sweeping M and B over the lane's blocks
-// in DESCENDING order, in place, every block still finds its left neighbour's row r-1 untouched; K then runs ASCENDING, in place, behind
-// the new M and B (and M has already used the old K).  The one-piece form kept a copy of each block's previous row for its right
-// neighbour: 9 of the step's 17 register moves.  Every cell's own operations and their order are unchanged.
+// lK_r): the block to the left in this row, (lM_p, ...): in the previous row), in two halves so that a step needs no copy of the previous
+// row.  The M and B cells of row r read row r-1 of their own block and of the block to the left; K reads row r of the block to the left.
+// Sweeping M and B over the lane's blocks in DESCENDING order, in place, every block still finds its left neighbour's row r-1 untouched; K
+// then runs ASCENDING, in place, behind the new M and B (and M has already used the old K).  The soft clip (block 0 of row 1) has no bit:
+// no other candidate of that cell is finite, its walk takes the move of "no bit set" (SAME_M) to row 0 and ends there.
+
+// x = 2 x + the sign of d, "this candidate is NOT the maximum" (the finished word is complemented): d = candidate - maximum is +0 or
+// negative.  (A cell without any path, everything -inf, gets the sign of a NaN: no walk comes there.)
+__device__ __forceinline__ uint32_t ea_push(const uint32_t x, const float d) { return __builtin_amdgcn_alignbit(x, __builtin_bit_cast(uint32_t, d), 31); }
 template <bool FIRST>
 __device__ __forceinline__ void ea_block_mb(float& M, float& B, const float lM_p, const float lB_p, const float lK_p, const float x, const np_gauss& g,
-                                            const ea_trans& tr, const float soft, uint64_t* __restrict__ p)
+                                            const ea_trans& tr, const float soft, uint32_t& word)
 {
     const float em = np_emission(x, g);
     const float a0 = tr.mm_self + M, a1 = tr.mm_next + lM_p, a2 = tr.bm_self + B, a3 = tr.bm_next + lB_p, a4 = tr.km + lK_p;
     float v = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(a0, a1), a2), a3), a4);      // two three-input maxima
     if (FIRST) v = __builtin_fmaxf(v, soft);
-    const uint64_t e1 = __builtin_amdgcn_ballot_w64(a1 == v), e2 = __builtin_amdgcn_ballot_w64(a2 == v), e3 = __builtin_amdgcn_ballot_w64(a3 == v),
-                   e4 = __builtin_amdgcn_ballot_w64(a4 == v);
-    const uint64_t t23 = e3 | e2, t234 = e4 | t23;
-    uint64_t c0 = t23 & ~e4, c1 = ~t234, c2 = (e4 | e3) | (e1 & c1);
-    if (FIRST) { const uint64_t es = __builtin_amdgcn_ballot_w64(soft == v); c0 |= es; c1 |= es; c2 |= es; }
+    word = ea_push(ea_push(ea_push(ea_push(word, a1 - v), a2 - v), a3 - v), a4 - v);
     const float newM = v + em;
     const float b0 = tr.mb + M, b2 = tr.bb + B;
     const float newB = __builtin_fmaxf(b0, b2);
-    const uint64_t pb = __builtin_amdgcn_ballot_w64(b2 >= b0);
+    word = ea_push(word, b2 - newB);
     M = newM; B = newB;
-    p[0] = c0; p[1] = c1; p[2] = c2; p[3] = ~pb;
 }
-__device__ __forceinline__ void ea_block_k(float& K, const float lM_r, const float lB_r, const float lK_r, const ea_trans& tr, uint64_t* __restrict__ p)
+__device__ __forceinline__ void ea_block_k(float& K, const float lM_r, const float lB_r, const float lK_r, const ea_trans& tr, uint32_t& word)
 {
     const float k1 = tr.mk + lM_r, k3 = tr.bk + lB_r, k4 = tr.kk + lK_r;
     const float newK = __builtin_fmaxf(__builtin_fmaxf(k1, k3), k4);
-    const uint64_t q4 = __builtin_amdgcn_ballot_w64(k4 == newK), q3 = __builtin_amdgcn_ballot_w64(k3 == newK);
+    word = ea_push(ea_push(word, k3 - newK), k4 - newK);
     K = newK;
-    p[4] = ~(q3 | q4); p[5] = q3 & ~q4;
-}
-// x = 64 x + the lane's bits of the six masks of a block (M high to low, B, K high to low: see the line's layout above).  One add with
-// carry per mask.  (The compiler does not look for hazards inside the block: the masks are scalar logic's results, and should it ever
-// put a compare's own result here, the two idle states are what a vector read of it needs.)
-__device__ __forceinline__ uint32_t ea_pack(uint32_t x, const uint64_t* __restrict__ p)
-{
-    asm("s_nop 1\n\t"
-        "v_addc_co_u32_e64 %0, vcc, %0, %0, %1\n\tv_addc_co_u32_e64 %0, vcc, %0, %0, %2\n\tv_addc_co_u32_e64 %0, vcc, %0, %0, %3\n\t"
-        "v_addc_co_u32_e64 %0, vcc, %0, %0, %4\n\tv_addc_co_u32_e64 %0, vcc, %0, %0, %5\n\tv_addc_co_u32_e64 %0, vcc, %0, %0, %6"
-        : "+v"(x) : "s"(p[2]), "s"(p[1]), "s"(p[0]), "s"(p[3]), "s"(p[4]), "s"(p[5]) : "vcc");
-    return x;
 }
 
 struct ea_seg { const float* ev; int e_start, stride, e, n; };
@@ -210,18 +187,16 @@ __device__ __attribute__((noinline)) float2 ea_fill2(const ea_gauss<BPL> G, cons
         const float x = xn;
         off0 += d0; off1 += d1;
         { const float xa = buf_f32(evr0, off0), xb = buf_f32(evr1, off1); xn = hi_half ? xb : xa; }
-        uint64_t pl[6 * BPL];
+        uint32_t wm = 0u, wk = 0u;
 #pragma unroll
-        for (int c = BPL - 1; c >= 1; --c) ea_block_mb<false>(M[c], B[c], M[c - 1], B[c - 1], K[c - 1], x, G.g[c], tr, NP_NEG_INF, pl + 6 * c);
-        ea_block_mb<true>(M[0], B[0], oM, oB, oK, x, G.g[0], tr, soft, pl);
-        ea_block_k(K[0], nM, nB, nK, tr, pl);
+        for (int c = BPL - 1; c >= 1; --c) ea_block_mb<false>(M[c], B[c], M[c - 1], B[c - 1], K[c - 1], x, G.g[c], tr, NP_NEG_INF, wm);
+        ea_block_mb<true>(M[0], B[0], oM, oB, oK, x, G.g[0], tr, soft, wm);
+        ea_block_k(K[0], nM, nB, nK, tr, wk);
 #pragma unroll
-        for (int c = 1; c < BPL; ++c) ea_block_k(K[c], M[c - 1], B[c - 1], K[c - 1], tr, pl + 6 * c);
+        for (int c = 1; c < BPL; ++c) ea_block_k(K[c], M[c - 1], B[c - 1], K[c - 1], tr, wk);
         oM = nM; oB = nB; oK = nK;
         soft = NP_NEG_INF;
-        uint32_t word = 0u;
-#pragma unroll
-        for (int c = BPL - 1; c >= 0; --c) word = ea_pack(word, pl + 6 * c);
+        const uint32_t word = ~((wk << (5 * BPL)) | wm);          // set: the candidate IS the maximum
         lines[(size_t)(t - 1) * (NP_EA2_LINE_BYTES / 4) + lane] = word;
     };
     int t = 1;
@@ -370,12 +345,14 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 struct ea_walk_result { int nb0, nb1, spilled0, spilled1; };       // bursts in all, bursts spilled
 
-// A walk step takes its move from the dword of the lane that owns the k-mer: bits pos .. pos + width - 1 of it plus a bias, by the state
-// walked in (0 KMER_SKIP, 1 BAD_EVENT, 2 MATCH); pos = 6 (k % BPL) + the state's first bit.  The three numbers of a state are bytes of
-// constants.
-#define NP_EA_FIRST 0x030200u
-#define NP_EA_WIDTH 0x030102u
-#define NP_EA_BIAS  0x000104u
+// A walk step takes its move from the dword of the lane that owns the k-mer: the state walked in (0 KMER_SKIP, 1 BAD_EVENT, 2 MATCH) has
+// its bits from pos = first bit + stride x (k % BPL) on; the lowest set one -- or the end mark behind the state's last bit -- is the
+// candidate, its move code three bits of NP_EA_CODES.  The numbers of a state are bytes of constants.
+#define NP_EA_POS0(BPL) (7u * (BPL) - 2u + 0x010000u)       // per state: first bit of block 0 (K 5 BPL + 2 (BPL - 1), B 0, M 1)
+#define NP_EA_STRIDE 0x0505fe            // per state: what a block adds to its first bit (5, 5, -2)
+#define NP_EA_END   0x100204u            // per state: the bit after its last candidate's
+#define NP_EA_ROW   0x0f0900u            // per state: first bit of its row of NP_EA_CODES
+#define NP_EA_CODES ((4u | 5u << 3 | 6u << 6) | (1u << 9 | 2u << 12) | (4u << 15 | 5u << 18 | 1u << 21 | 6u << 24 | 2u << 27))
 
 // the lane (of its half) that owns k-mer k = k / BPL, as full-rate instructions (a 32-bit multiply-high is quarter rate); 5 bits, as the
 // shifts that use it take
@@ -385,6 +362,12 @@ __device__ __forceinline__ uint32_t ea_mul24(const uint32_t a, const uint32_t b)
 {
     uint32_t p;
     asm("v_mul_u32_u24 %0, %1, %2" : "=v"(p) : "v"(a), "v"(b));
+    return p;
+}
+__device__ __forceinline__ uint32_t ea_mad24(const uint32_t a, const int b, const uint32_t c)
+{
+    uint32_t p;
+    asm("v_mad_i32_i24 %0, %1, %2, %3" : "=v"(p) : "v"(a), "v"(b), "v"(c));
     return p;
 }
 template <int BPL> __device__ __forceinline__ uint32_t ea_owner(const uint32_t k)
@@ -468,13 +451,15 @@ __device__ __attribute__((noinline)) ea_walk_result ea_walk2(ea_lds* L, const fl
         uint64_t am = __builtin_amdgcn_ballot_w64(alive); // inside the burst "alive" is this scalar mask, the counts scalar additions
         for (int s = 0; s < burst; ++s) {
             steps0 += (uint32_t)am & 1u; steps1 += (uint32_t)(am >> 32) & 1u;
-            // the move out of this cell: the dword of the lane that owns the k-mer, of it the state's field of the k-mer's block
+            // the move out of this cell: the dword of the lane that owns the k-mer, of it the state's bits of the k-mer's block
             const uint32_t own = ea_owner<BPL>((uint32_t)k);
             const uint32_t off = ea_mul24(own, 4u * NP_EA_LDW + 4u) + (((uint32_t)row * (4u * NP_EA_LDW)) - lo128);
             const uint32_t w = *(const lds_u32*)(st + (off < (uint32_t)(4 * (WIN * NP_EA_LDW - 1)) ? off : (uint32_t)(4 * (WIN * NP_EA_LDW - 1))));
             const uint32_t b8 = (uint32_t)ps * 8u;
-            const uint32_t pos = ea_mul24((uint32_t)k - ea_mul24(own, BPL), 6u) + __builtin_amdgcn_ubfe(NP_EA_FIRST, b8, 8);
-            const uint32_t c = __builtin_amdgcn_ubfe(w, pos, __builtin_amdgcn_ubfe(NP_EA_WIDTH, b8, 8)) + __builtin_amdgcn_ubfe(NP_EA_BIAS, b8, 8);
+            const uint32_t blk = (uint32_t)k - ea_mul24(own, BPL);
+            const uint32_t pos = ea_mad24(blk, __builtin_amdgcn_sbfe(NP_EA_STRIDE, b8, 8), __builtin_amdgcn_ubfe(NP_EA_POS0(BPL), b8, 8));
+            const uint32_t f = (w >> (pos & 31u)) | __builtin_amdgcn_ubfe(NP_EA_END, b8, 8);
+            const uint32_t c = __builtin_amdgcn_ubfe(NP_EA_CODES, (uint32_t)__builtin_ctz(f) * 3u + __builtin_amdgcn_ubfe(NP_EA_ROW, b8, 8), 3);
             codes |= c << (3 * s);
             row -= ps != 0 ? 1 : 0;                                     // K states are silent (r9.cpp:176-178)
             k -= (int)(c >> 2);
