@@ -837,7 +837,17 @@ __global__ void __launch_bounds__(64, 3) np_ed_peaks_par_kernel(int n_reads, con
     const bool over = __builtin_amdgcn_ballot_w64(cnt > tmp_cap) != 0ull || total + 1 > cap;
     if (!over) {
         if (lane == 0) es[0] = 0u;
-        for (int q = 0; q < cnt; ++q) es[1 + off + q] = tmp[q];
+        // (eight at a time, by hand: entry by entry the copy is one memory round trip per peak and a third of the kernel's time -- 18.1 against
+        //  27.0 ms per 50 000 reads; the compiler's vectoriser only forms such a loop where packed fp32 is allowed)
+        int q = 0;
+        for (; q + 8 <= cnt; q += 8) {
+            uint32_t v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = tmp[q + u];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) es[1 + off + q + u] = v[u];
+        }
+        for (; q < cnt; ++q) es[1 + off + q] = tmp[q];
     }
     if (lane == 0) n_events[r] = over ? NP_ED_OVERFLOW : (total > 0 ? total + 1 : 0);
 }

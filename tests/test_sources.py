@@ -2,6 +2,9 @@
 import glob
 import os
 import re
+import subprocess
+
+import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 DIRS = ["nanopolish_amd/csrc", "tools"]
@@ -28,3 +31,22 @@ def test_scalar_instructions_in_inline_assembly_do_not_write_memory():
                 continue
             for w in re.findall(r"(?:(?<=^)|(?<=\\n)|(?<=\\t)|(?<=\s))(s_[a-z0-9_]+)", lit):
                 assert ok.fullmatch(w), (os.path.relpath(f, ROOT), w)
+
+
+def _makefile_flags():
+    text = open(os.path.join(ROOT, "nanopolish_amd", "csrc", "Makefile")).read()
+    return re.search(r"^CXXFLAGS = (.*)$", text, re.M).group(1).replace("$(ARCH)", "gfx950").split()
+
+
+def test_the_product_is_built_without_packed_fp32(tmp_path):
+    """The compiler makes packed fp32 instructions from ordinary float code; the Makefile's flags keep them out of the device code (the event
+    detector's translation unit is the one where it finds pairs)."""
+    hipcc = "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("no hipcc")
+    out = str(tmp_path / "events.s")
+    subprocess.run([hipcc] + _makefile_flags() + ["-S", "--cuda-device-only", os.path.join(ROOT, "nanopolish_amd", "csrc", "np_events_kernels.hip"), "-o", out],
+                   check=True, capture_output=True)
+    text = open(out).read()
+    assert "v_add_f32" in text
+    assert re.findall(r"\bv_pk_(?:add|mul|fma)_f32\b", text) == []

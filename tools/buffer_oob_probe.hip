@@ -1,6 +1,6 @@
 // Probe: what does a range-checked raw buffer load of 8 bytes return when only ONE of its two dwords is in range?
 // (decides whether kernel A may fetch the event means of a lane's two adjacent slots with one buffer_load_dwordx2)
-//   hipcc --offload-arch=gfx950 -O2 tools/buffer_oob_probe.hip -o tools/buffer_oob_probe && tools/buffer_oob_probe
+//   hipcc -O2 -Xclang -target-feature -Xclang -packed-fp32-ops --offload-arch=gfx950 tools/buffer_oob_probe.hip -o tools/buffer_oob_probe && tools/buffer_oob_probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

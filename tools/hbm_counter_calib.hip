@@ -6,7 +6,7 @@
 //   calib_read16  coalesced 16 B/lane loads  (the guide's calibrated case; kernel A: parameter records)
 //   calib_write4  coalesced 4 B/lane stores  (kernel A: packed trace)
 //   calib_write8  coalesced 8 B/lane stores  (kernel A: AlignedPair lists)
-//   hipcc --offload-arch=gfx950 -O2 tools/hbm_counter_calib.hip -o tools/hbm_counter_calib
+//   hipcc -O2 -Xclang -target-feature -Xclang -packed-fp32-ops --offload-arch=gfx950 tools/hbm_counter_calib.hip -o tools/hbm_counter_calib
 //   rocprofv3 --kernel-trace --pmc FETCH_SIZE ... -- tools/hbm_counter_calib     (and a second pass with WRITE_SIZE)
 #include <hip/hip_runtime.h>
 #include <cstdio>

@@ -8,7 +8,7 @@
 //   2. exact    -- D == C + B bit for bit against v_add_f64 (random operands, -inf / huge / tiny in C, finite B);
 //   3. rates    -- SIMD cycles per wave-instruction of the MFMA alone, and of a band-like VALU mix with its ten fp64 additions
 //                  on the vector port, on the matrix pipe, and removed (the most the move can give), at 8 waves per SIMD.
-// Build + run:  hipcc -O3 --offload-arch=gfx950 tools/mfma_f64_probe.hip -o /tmp/mfma_f64_probe && /tmp/mfma_f64_probe
+// Build + run:  hipcc -O3 -Xclang -target-feature -Xclang -packed-fp32-ops --offload-arch=gfx950 tools/mfma_f64_probe.hip -o /tmp/mfma_f64_probe && /tmp/mfma_f64_probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

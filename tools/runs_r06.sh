@@ -13,7 +13,7 @@ cd "$GRAFT_REPO_ROOT" || exit 1
 O=gpurun_out/r06b; mkdir -p $O
 ( time timeout 1200 python -m pytest tests -m gpu -x -q ) > $O/pytest.log 2>&1; echo "pytest rc=$?" >> $O/pytest.log
 ./tools/mfma_f64_probe > $O/probe.log 2>&1
-/opt/rocm/bin/hipcc -O2 --offload-arch=gfx950 tools/valu_rates.hip -o /tmp/valu_rates > /dev/null 2>&1 && /tmp/valu_rates l > $O/valu_l.log 2>&1
+/opt/rocm/bin/hipcc -O2 -Xclang -target-feature -Xclang -packed-fp32-ops --offload-arch=gfx950 tools/valu_rates.hip -o /tmp/valu_rates > /dev/null 2>&1 && /tmp/valu_rates l > $O/valu_l.log 2>&1
 ( timeout 900 python tools/align_ab.py --pool 2048 --tile 16 $V/libnp_hip_base.so $V/libnp_hip_m0sel.so $V/libnp_hip_base.so $V/libnp_hip_m0sel.so ) > $O/align_ab.log 2>&1
 ( time timeout 600 python bench.py --steps 5 --warmup 2 --legs 0 --streamed 0 --ragged 0 --cpu-sample 0 ) > $O/bench.json 2> $O/bench.err
 tail -5 $O/pytest.log; grep "waves/SIMD 8" $O/probe.log; cat $O/valu_l.log; cat $O/align_ab.log; head -c 600 $O/bench.json; tail -3 $O/bench.err

@@ -1,7 +1,7 @@
 // valu_rates.hip -- issue cost (cycles per wave-instruction) of the VALU ops the two kernels are made of, measured on
 // the device with s_memtime around long independent instruction streams.  One wave per SIMD (no contention), 8
 // independent destination registers per op so that latency does not limit issue.  Build + run:
-//   hipcc -O2 --offload-arch=gfx950 tools/valu_rates.hip -o /tmp/valu_rates && /tmp/valu_rates
+//   hipcc -O2 -Xclang -target-feature -Xclang -packed-fp32-ops --offload-arch=gfx950 tools/valu_rates.hip -o /tmp/valu_rates && /tmp/valu_rates
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
