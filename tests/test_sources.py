@@ -50,3 +50,9 @@ def test_the_product_is_built_without_packed_fp32(tmp_path):
     text = open(out).read()
     assert "v_add_f32" in text
     assert re.findall(r"\bv_pk_(?:add|mul|fma)_f32\b", text) == []
+
+
+def test_no_packed_fp32_by_hand():
+    for f in _gpu_sources():
+        for lit in re.findall(r'"((?:[^"\\\n]|\\.)*)"', open(f).read()):
+            assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", lit), (os.path.relpath(f, ROOT), lit)

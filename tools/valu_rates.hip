@@ -26,8 +26,6 @@ template <int OP> __global__ void k(unsigned long long* out, float* sink, int it
 #define CVT32(n) asm volatile("v_cvt_f32_f64 %0, %1" : "=v"(a##n) : "v"(d##n));
 #define ADD64(n) asm volatile("v_add_f64 %0, %1, %1" : "=v"(d##n) : "v"(d##n));
 #define FMA32(n) asm volatile("v_fma_f32 %0, %1, %1, %1" : "=v"(a##n) : "v"(a##n));
-#define PKFMA(n) asm volatile("v_pk_fma_f32 %0, %1, %1, %1" : "=v"(p##n) : "v"(p##n));
-#define PKMUL(n) asm volatile("v_pk_mul_f32 %0, %1, %1" : "=v"(p##n) : "v"(p##n));
 #define MAX3(n) asm volatile("v_max3_f32 %0, %1, %1, %1" : "=v"(a##n) : "v"(a##n));
 #define CNDM(n) asm volatile("v_cndmask_b32 %0, %1, %1, vcc" : "=v"(a##n) : "v"(a##n));
 #define DPPM(n) asm volatile("v_mov_b32_dpp %0, %1 wave_ror:1 row_mask:0xf bank_mask:0xf" : "=v"(a##n) : "v"(a##n));
@@ -39,7 +37,6 @@ template <int OP> __global__ void k(unsigned long long* out, float* sink, int it
 #define CNDV2(n) asm volatile("v_cndmask_b32 %0, %1, %2, vcc" : "=v"(a##n) : "v"(a##n), "v"(a0));
 #define SUBU(n) asm volatile("v_sub_u32 %0, %1, %1" : "=v"(a##n) : "v"(a##n));
 #define MAXF(n) asm volatile("v_max_f32 %0, %1, %1" : "=v"(a##n) : "v"(a##n));
-#define PKADD(n) asm volatile("v_pk_add_f32 %0, %1, %1" : "=v"(p##n) : "v"(p##n));
 #define MOVB(n) asm volatile("v_mov_b32 %0, %1" : "=v"(a##n) : "v"(a##n));
 #define FMA3(n) asm volatile("v_fma_f32 %0, %1, %2, %3" : "=v"(a##n) : "v"(a##n), "v"(a0), "v"(a1));
 #define MAX3D(n) asm volatile("v_max3_f32 %0, %1, %2, %3" : "=v"(a##n) : "v"(a##n), "v"(a0), "v"(a1));
@@ -140,8 +137,6 @@ template <int OP> __global__ void k(unsigned long long* out, float* sink, int it
         if (OP == 1) { REP8(CVT32) REP8(CVT32) }
         if (OP == 2) { REP8(ADD64) REP8(ADD64) }
         if (OP == 3) { REP8(FMA32) REP8(FMA32) }
-        if (OP == 4) { REP8(PKFMA) REP8(PKFMA) }
-        if (OP == 5) { REP8(PKMUL) REP8(PKMUL) }
         if (OP == 6) { REP8(MAX3) REP8(MAX3) }
         if (OP == 7) { REP8(CNDM) REP8(CNDM) }
         if (OP == 8) { REP8(DPPM) REP8(DPPM) }
@@ -201,7 +196,6 @@ template <int OP> __global__ void k(unsigned long long* out, float* sink, int it
         if (OP == 17) { REP8(CNDV2) REP8(CNDV2) }
         if (OP == 18) { REP8(SUBU) REP8(SUBU) }
         if (OP == 19) { REP8(MAXF) REP8(MAXF) }
-        if (OP == 20) { REP8(PKADD) REP8(PKADD) }
         if (OP == 21) { REP8(MOVB) REP8(MOVB) }
         if (OP == 22) { REP8(FMA3) REP8(FMA3) }
         if (OP == 23) { REP8(MAX3D) REP8(MAX3D) }
@@ -292,7 +286,7 @@ int main(int argc, char** argv)
     }
     for (int w : {8, 4, 2, 1}) {
         if (argc > 1) break;          // any argument: only the round-2 table
-        run<12>("v_add_f32", w); run<3>("v_fma_f32", w); run<4>("v_pk_fma_f32", w); run<5>("v_pk_mul_f32", w);
+        run<12>("v_add_f32", w); run<3>("v_fma_f32", w);
         run<0>("v_cvt_f64_f32", w); run<1>("v_cvt_f32_f64", w); run<16>("v_cvt_f64_u32", w); run<2>("v_add_f64", w);
         run<15>("v_mul_f64", w); run<11>("v_fma_f64", w);
         run<6>("v_max3_f32", w); run<7>("v_cndmask_b32", w); run<8>("v_mov_dpp ror", w); run<9>("v_readlane", w);
@@ -304,7 +298,7 @@ int main(int argc, char** argv)
         run<40>("v_cvt_u32_f32", w); run<41>("v_cvt_i32_f32", w); run<42>("v_min_u32", w); run<43>("v_min_f32", w); run<44>("v_mul_f32", w);
         run<45>("v_mul_f32 |abs|", w); run<46>("v_lshlrev_b32", w); run<47>("v_and_b32", w); run<48>("ds_read_b32", w); run<49>("v_med3_i32", w);
         run<50>("v_max_i32", w); run<51>("v_sub_f32", w); run<52>("v_add_u32", w); run<53>("v_lshl_add_u32", w);
-        run<20>("v_pk_add_f32", w); run<21>("v_mov_b32", w); run<22>("v_fma_f32 3src", w); run<23>("v_max3 3src", w);
+        run<21>("v_mov_b32", w); run<22>("v_fma_f32 3src", w); run<23>("v_max3 3src", w);
     }
     // round 2 table (per 16 instructions of the named kind; pairs / sequences are marked)
     for (int w : {8}) {
