@@ -1,4 +1,5 @@
 """Rules that the GPU sources follow by themselves, checked on the text (CPU)."""
+import ast
 import glob
 import os
 import re
@@ -56,3 +57,15 @@ def test_no_packed_fp32_by_hand():
     for f in _gpu_sources():
         for lit in re.findall(r'"((?:[^"\\\n]|\\.)*)"', open(f).read()):
             assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", lit), (os.path.relpath(f, ROOT), lit)
+
+
+def test_streams_keep_the_default_priority():
+    """Work on streams of different priorities has hung here for good: no stream or process group asks for one."""
+    files = [f for d in ("", "nanopolish_amd", "tools", "tests", "oracle") for f in glob.glob(os.path.join(ROOT, d, "*.py"))]
+    assert len(files) > 40
+    for f in files:
+        for node in ast.walk(ast.parse(open(f).read())):
+            if isinstance(node, ast.Call):
+                assert not {k.arg for k in node.keywords} & {"priority", "is_high_priority_stream"}, (os.path.relpath(f, ROOT), node.lineno)
+    for f in _gpu_sources() + glob.glob(os.path.join(ROOT, "nanopolish_amd", "csrc", "*.cpp")):
+        assert "StreamCreateWithPriority" not in open(f).read(), f

@@ -44,8 +44,8 @@ def main():
                 b.sync()
             torch.cuda.synchronize()
 
-        def run(mode, prio=False, skew_ms=0.0):
-            sts = [torch.cuda.Stream(priority=(-1 if (prio and i % 2) else 0)) for i in range(P)]
+        def run(mode, skew_ms=0.0):
+            sts = [torch.cuda.Stream() for i in range(P)]
             for i, b in enumerate(batches):
                 b.stream = sts[0].cuda_stream if mode == "one" else sts[i].cuda_stream
             for b in batches:        # warm-up round (and the initial skew between the parts)
@@ -60,7 +60,7 @@ def main():
                     b.step()
             sync_all()
             dt = time.perf_counter() - t
-            return dict(parts=P, mode=mode, prio=prio, skew_ms=skew_ms, reads_per_round=n_reads, ms_per_round=round(1e3 * dt / args.steps, 2),
+            return dict(parts=P, mode=mode, skew_ms=skew_ms, reads_per_round=n_reads, ms_per_round=round(1e3 * dt / args.steps, 2),
                         reads_per_s=round(n_reads * args.steps / dt, 1))
 
         def run_stages(wa, wb):
@@ -98,7 +98,6 @@ def main():
             print(json.dumps(run("streams")), flush=True)
             print(json.dumps(run("streams", skew_ms=step_ms / P / 2)), flush=True)
             print(json.dumps(run("streams", skew_ms=step_ms / P)), flush=True)
-            print(json.dumps(run("streams", prio=True, skew_ms=step_ms / P)), flush=True)
         sc = np.concatenate([b.scores()[: 2 * 1000] for b in batches[:1]])
         if ref_scores is None:
             ref_scores = sc
