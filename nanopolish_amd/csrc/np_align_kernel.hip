@@ -680,7 +680,12 @@ __global__ void __launch_bounds__(NP_ALIGN_BLOCK, NP_A_WAVES) np_event_align_ker
                     }
                 }
 #undef NP_BT_LOAD
+                // the walk leaves with up to NP_BT_DEPTH requests in flight: the queue's registers belong to them until they have landed, and
+                // each is used once more behind the wait (an output nobody uses any more would be a free register to the compiler, and the
+                // load would write into whatever it put there)
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < NP_BT_DEPTH; ++i) asm volatile("" : "+v"(tq[i]));
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
                 // QC sum (:338-341) over the stored pairs, 64 at a time.  The reference adds the emissions in walk order; only
                 // the comparison of their mean with the threshold is used.  Any summation order of n doubles is within
