@@ -57,11 +57,6 @@
 #ifndef NP_A_WAVES
 #define NP_A_WAVES 8      // resident waves per SIMD the register budget is set for
 #endif
-// timing experiments only (results are WRONG with any bit set): 1 no trace, 2 fp32 candidate sums, 4 fixed move pattern (no band-end
-// reads, no scalar decision chain), 16 trivial emission, 128 no back-track
-#ifndef NP_ABL
-#define NP_ABL 0
-#endif
 #ifndef NP_A_WALK_PRIO
 #define NP_A_WALK_PRIO 3  // wave priority during the back-track (s_setprio): a dependent scalar chain that needs few issue slots but holds a
 #endif                    // wave slot for as long as it takes; 45.6 -> 43.2 ms per 32768 reads
@@ -266,12 +261,8 @@ __device__ __forceinline__ void band_step(fill_t& F, const read_t& R, const int 
 
     // emissions of both cells: np_emission / np_div_exact, operation for operation (v_pk_*_f32 would halve the
     // instruction count but not the issue cycles -- tools/valu_rates.hip -- and forces the parameters into register pairs)
-#if NP_ABL & 16
-    const float emx = x0 * F.g0.z, emy = x1 * F.g1.z;
-#else
     const float emx = np_emission_nd(x0, F.g0.x, F.g0.y, F.g0.z, F.g0.w);
     const float emy = np_emission_nd(x1, F.g1.x, F.g1.y, F.g1.z, F.g1.w);
-#endif
     // stand-alone step: the next band's event means go into the registers the emissions have just released: the loop-carried
     // value is the load's own destination, so nothing is copied (a copy would have to wait for the load)
     if (POS < 0) {
@@ -282,22 +273,11 @@ __device__ __forceinline__ void band_step(fill_t& F, const read_t& R, const int 
     // DP cells (raw_loader.cpp:240-289), computed unconditionally and masked: fp32 cell + fp64 constant + fp32 emission
     // in fp64, rounded to fp32; max, then FROM_U / FROM_L override on equality in that order (later candidate wins).
     // (double)p0 is `up` of the even slot AND `left` of the odd one; the two `left` doubles are the next band's diagonals.
-#if NP_ABL & 2
-    const double P0 = (double)F.p0, L0 = (double)l0;
-    const float sd0 = (float)F.d0 + (float)R.lp_step + emx, sd1 = (float)F.d1 + (float)R.lp_step + emy;
-    const float su0 = F.p0 + (float)R.lp_stay + emx, su1 = F.p1 + (float)R.lp_stay + emy;
-    const float sl0 = l0 + (float)R.lp_skip, sl1 = F.p0 + (float)R.lp_skip;
-#else
     const double em0 = (double)emx, em1 = (double)emy;
     const double P0 = (double)F.p0, P1 = (double)F.p1, L0 = (double)l0;
     const float sd0 = (float)(F.d0 + R.lp_step + em0), sd1 = (float)(F.d1 + R.lp_step + em1);
     const float su0 = (float)(P0 + R.lp_stay + em0), su1 = (float)(P1 + R.lp_stay + em1);
-#if NP_ABL & 32
-    const float sl0 = NP_NEG_INF, sl1 = NP_NEG_INF;      // timing experiment only (results WRONG): the left (k-mer skip) candidates for free
-#else
     const float sl0 = (float)(L0 + R.lp_skip), sl1 = (float)(P0 + R.lp_skip);
-#endif
-#endif
     const float m0 = __builtin_fmaxf(__builtin_fmaxf(sd0, su0), sl0);
     const float m1 = __builtin_fmaxf(__builtin_fmaxf(sd1, su1), sl1);
 
@@ -305,7 +285,7 @@ __device__ __forceinline__ void band_step(fill_t& F, const read_t& R, const int 
     // so that the scalar chain of the move decision runs while the vector unit packs.  (The ends are inside the window:
     // the unmasked maxima are the cells.)
     int xs = 0, ys = 0;
-    if (FAST && !(NP_ABL & 4)) {
+    if (FAST) {
 #if NP_A_FILL_PRIO
         if (POS >= 0) __builtin_amdgcn_s_setprio(NP_A_FILL_PRIO);
 #endif
@@ -327,7 +307,6 @@ __device__ __forceinline__ void band_step(fill_t& F, const read_t& R, const int 
         // pads with s_nop): the four compares write four scalar pairs, and by the time an add-with-carry shifts a mask into the
         // accumulator three other instructions have issued.
         uint64_t qa, qb, qc, qd, qj;
-#if !(NP_ABL & 1)
         asm("v_cmp_eq_f32_e64 %[a], %[m1], %[l1]\n\t"
             "v_cmp_eq_f32_e64 %[b], %[m1], %[u1]\n\t"
             "v_cmp_eq_f32_e64 %[c], %[m0], %[l0]\n\t"
@@ -338,7 +317,6 @@ __device__ __forceinline__ void band_step(fill_t& F, const read_t& R, const int 
             "v_addc_co_u32_e64 %[t], %[j], %[t], %[t], %[d]"
             : [t] "+v"(F.tacc), [a] "=&s"(qa), [b] "=&s"(qb), [c] "=&s"(qc), [d] "=&s"(qd), [j] "=&s"(qj)
             : [m0] "v"(m0), [u0] "v"(su0), [l0] "v"(sl0), [m1] "v"(m1), [u1] "v"(su1), [l1] "v"(sl1));
-#endif
     }
     uint32_t f0 = 0u, f1 = 0u;
     if (!FAST) {
@@ -363,11 +341,9 @@ __device__ __forceinline__ void band_step(fill_t& F, const read_t& R, const int 
     // packed trace: every lane keeps the bits of its two slots, 4 bits per band, and stores one dword per 8 bands
     // (64 lanes x 4 B = 256 B coalesced = 32 B/band).  The back-track reads the word back into the SAME lane.
     // (the word shifts up one nibble per band, so after 8 bands band b%8 == 0 sits in bits 31..28: no variable shift)
-#if !(NP_ABL & 1)
     if (!FAST) F.tacc = (F.tacc << 4) | (f1 << 2) | f0;
     if (POS == 1 ? (b & 7) == 7 : (POS < 0 && (b & 7) == 7))
         __builtin_amdgcn_raw_buffer_store_b32((int)F.tacc, R.tr, 4 * lane, (pin_s(b) >> 3) * 256, 0);    // (pin_s: no second induction variable)
-#endif
 
     if (END && khi == K - 1 && llk <= K - 1) {
         // end search: cell (e, K-1) while it is inside the window, any e in [0,E) (:309-324).  Wave-uniform: the cell's ring
@@ -383,7 +359,7 @@ __device__ __forceinline__ void band_step(fill_t& F, const read_t& R, const int 
     F.d0 = L0; F.d1 = P0;
     F.p0 = c0; F.p1 = c1;
 
-    if (FAST && POS >= 0 && !(NP_ABL & 4)) {
+    if (FAST && POS >= 0) {
         // Suzuki's rule (see below) in the pair loop, where the band's parity is known.  ll < ur for floats that are +0, negative
         // or -inf (R.nonpos) is bits(ll) > bits(ur) as unsigned integers; "both ends -inf: alternate, right on even bands" needs
         // nothing on odd bands (equal patterns compare false) and on even bands is the same compare against min(ur, bits(-FLT_MAX)):
@@ -407,9 +383,7 @@ __device__ __forceinline__ void band_step(fill_t& F, const read_t& R, const int 
         // then): alternate; else right iff ll < ur, where a single -inf compares as the reference's
         // is_offset_valid ? value : -INFINITY does
         bool right;
-        if (FAST && (NP_ABL & 4)) {
-            right = (((b + 1) * 13) >> 5) != ((b * 13) >> 5);       // a fixed pattern with the same share of right moves
-        } else if (FAST) {
+        if (FAST) {
             // FAST runs only for reads whose cells are all <= 0 (R.nonpos): for such floats (+0, negative, -inf) x < y is
             // bits(x) > bits(y) as unsigned integers -- scalar compares instead of a vector compare on two scalars
             // (spelled out for the scalar unit: hipcc lowers a select between wave-uniform conditions to vector code)
@@ -573,7 +547,7 @@ __global__ void __launch_bounds__(NP_ALIGN_BLOCK, NP_A_WAVES) np_event_align_ker
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
             __builtin_amdgcn_s_waitcnt(0);
 
-            if (best_u != NP_NEG_INF && !(NP_ABL & 128)) {
+            if (best_u != NP_NEG_INF) {
 #if NP_A_WALK_PRIO
                 __builtin_amdgcn_s_setprio(NP_A_WALK_PRIO);
 #endif

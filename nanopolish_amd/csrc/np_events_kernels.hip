@@ -446,11 +446,6 @@ __device__ __forceinline__ float tstat_from_sums_fast(double sum1, double sumsq1
     return ed_ratio_filtered(delta_mean, cvw, near);      // (the caller applies compute_tstat's boundary rule and, where `near`, ed_ratio_exact)
 }
 
-#if defined(NP_ED_ABL) && (NP_ED_ABL & 4)
-#define NP_ED_ABL_NOSTORE && false      /* timing ablation: the per-lane event list is not written */
-#else
-#define NP_ED_ABL_NOSTORE
-#endif
 struct detector { int masked_to, peak_pos; float peak_value; int valid_peak; };
 
 template <int K>
@@ -631,12 +626,7 @@ __device__ __forceinline__ void walk_segment_raw(__amdgpu_buffer_rsrc_t xr, int 
     const int n_blk = (trip + 7) / 8 + 1;                     // a misaligned range of `trip` samples touches at most this many
     float W[24];                                              // blocks blk-1, blk, blk+1
     auto load_block = [&](int b, float* dst) {
-#ifdef NP_ED_ABL      // timing ablation (results wrong): bit 1 = no sample loads at all, bit 2 = every lane reads the SAME segment (coalesced, cached)
-        const bool need = !(NP_ED_ABL & 1) && lane_active && b >= 0 && b * 8 < n;
-        if (NP_ED_ABL & 2) b = b % 96;
-#else
         const bool need = lane_active && b >= 0 && b * 8 < n;
-#endif
         if (ADC) {
             // samples [8 b, 8 b + 8) = bytes [16 b + 2 lead, + 16) of the word-aligned stream
             uint32_t d0 = 0u, d1 = 0u, d2 = 0u, d3 = 0u, d4 = 0u;
@@ -708,11 +698,11 @@ __device__ __forceinline__ void walk_segment_raw(__amdgpu_buffer_rsrc_t xr, int 
                 const float t1 = w1 < w2 ? ta : tb, t2 = w1 < w2 ? tb : ta;
                 int pos;
                 if (detector_step<0>(st.d0, st.d1, in ? i : -1, t1, p.peak_height, p.threshold1, w1, pos) && RECORD) {
-                    if (cnt < tmp_cap NP_ED_ABL_NOSTORE) tmp[cnt] = (uint32_t)pos;
+                    if (cnt < tmp_cap) tmp[cnt] = (uint32_t)pos;
                     cnt++;
                 }
                 if (detector_step<1>(st.d1, st.d0, in ? i : -1, t2, p.peak_height, p.threshold2, w2, pos) && RECORD) {
-                    if (cnt < tmp_cap NP_ED_ABL_NOSTORE) tmp[cnt] = (uint32_t)pos;
+                    if (cnt < tmp_cap) tmp[cnt] = (uint32_t)pos;
                     cnt++;
                 }
                 // S(i + 4) = S(i + 3) - x[i+3] + x[i+6]
@@ -743,11 +733,11 @@ __device__ __forceinline__ void walk_segment_raw(__amdgpu_buffer_rsrc_t xr, int 
             const float t1 = w1 < w2 ? ta : tb, t2 = w1 < w2 ? tb : ta;
             int pos;
             if (detector_step<0>(st.d0, st.d1, in ? i : -1, t1, p.peak_height, p.threshold1, w1, pos) && RECORD) {
-                if (cnt < tmp_cap NP_ED_ABL_NOSTORE) tmp[cnt] = (uint32_t)pos;
+                if (cnt < tmp_cap) tmp[cnt] = (uint32_t)pos;
                 cnt++;
             }
             if (detector_step<1>(st.d1, st.d0, in ? i : -1, t2, p.peak_height, p.threshold2, w2, pos) && RECORD) {
-                if (cnt < tmp_cap NP_ED_ABL_NOSTORE) tmp[cnt] = (uint32_t)pos;
+                if (cnt < tmp_cap) tmp[cnt] = (uint32_t)pos;
                 cnt++;
             }
             // S(i + 4) = S(i + 3) - x[i+3] + x[i+6]

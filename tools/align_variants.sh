@@ -8,5 +8,4 @@ v all      ""
 v u8off    "-DNP_A_UNROLL8=0"
 v cmpxoff  "-DNP_A_CMPX=0"
 v traceoff "-DNP_A_TRACEASM=0"
-v nobt     "-DNP_ABL=128"
 ls ../variants/*.so | wc -l
