@@ -85,8 +85,8 @@ const char* np_ctx_info(const np_ctx* ctx);
  * "recal_shape" (np_calibrate_resolve_dev's workgroup shape, 3: the default -- sixteen waves x four reads, 32-k-mer chunks --, 0 ... 2: the shapes it was measured against; results never depend on it), "small_batch_path"
  * (1: np_hmm_score_host sends a small batch as one pinned blob; 0: the general path -- the tests compare the two).
  * Environment, read at np_create (each the option of the same name): NP_ALIGN_BLOCKS_PER_CU, NP_HMM_BLOCKS_PER_CU, NP_ALIGN_LPT, NP_ED_WARMUP, NP_ED_RATIO_EXACT,
- * NP_EA_WAVES_PER_CU, NP_RECAL_SHAPE; NP_EA_WALK_PRIO=1 runs the chain kernel's back-track at wave priority 3 (measured slower,
- * profiles/r05_soak.md); NP_LSE_CLAMP, NP_HOST_CONSTANTS (0 is refused), NP_VERBOSE as described at np_ctx_info / in INTEGRATION.md. */
+ * NP_EA_WAVES_PER_CU, NP_RECAL_SHAPE; NP_EA_WALK_PRIO=0 runs the chain kernel's back-track at the wave priority of the rest (229 against
+ * 222 ms per 50 000 reads); NP_LSE_CLAMP, NP_HOST_CONSTANTS (0 is refused), NP_VERBOSE as described at np_ctx_info / in INTEGRATION.md. */
 int np_set_option(np_ctx* ctx, const char* name, int64_t value);
 /* Read-only facts about the context (-1: unknown name): "align_blocks" / "align_scratch_bytes" (persistent grid and per-wave scratch
  * of the most recent event-align launch: the grid shrinks under a 48 GB scratch budget when a batch holds ultra-long reads),

@@ -464,9 +464,8 @@ __device__ __attribute__((noinline)) ea_walk_result ea_walk2(ea_lds* L, const fl
             row -= ps != 0 ? 1 : 0;                                     // K states are silent (r9.cpp:176-178)
             k -= (int)(c >> 2);
             ps = (int)(c & 3u);
-            // the walk ends at row 0 or k-mer -1.  (HMT_FROM_SOFT, code 7, is the move out of MATCH of (row 1, k-mer 0) only -- the one
-            // cell the sweep offers the soft clip to, ea_fill2 -- and leads to row 0: no test of its own.  A finished walk's row, k and
-            // state are not used again.)
+            // the walk ends at row 0 or k-mer -1 (the soft clip leads to row 0: no test of its own).  A finished walk's row, k and state are
+            // not used again.
             am &= __builtin_amdgcn_ballot_w64(row > 0) & __builtin_amdgcn_ballot_w64(k >= 0);      // (two ballots: each is its compare's own result register)
         }
         alive = __builtin_amdgcn_inverse_ballot_w64(am);
