@@ -912,8 +912,8 @@ def main():
         a_avg_s = a_ms / max(a_n, 1) * 1e-3
         algo = res["algo"]
         achieved = algo / a_avg_s / 1e9 if a_avg_s > 0 else 0.0
-        # HBM traffic of THIS run's launch: bytes per BAND from the counter passes over the shipped kernel (profiles/r04_pmc.json:
-        # rocprofv3 --pmc FETCH_SIZE / WRITE_SIZE at a launch size the passes finish at, profiles/collect_r04_pmc.sh) x the bands this
+        # HBM traffic of THIS run's launch: bytes per BAND from the counter passes over the shipped kernel (profiles/pmc_shipped.json:
+        # rocprofv3 --pmc FETCH_SIZE / WRITE_SIZE at a launch size the passes finish at, profiles/collect_r06_pmc.sh) x the bands this
         # run's reads have -- a from-raw run (more events per read) reports its own figure.  `issue`: vector instructions per band from
         # the same passes, priced at the calibrated issue cycles per class (profiles/r04_valu_calibration.json), over this run's
         # SIMD-cycles per band: floor = every instruction at the fastest class's cost, priced = by the class mix of the band loop.

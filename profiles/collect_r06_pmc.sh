@@ -5,13 +5,14 @@
 # One process per pass (rocprofv3 --pmc only together with --kernel-trace; FETCH_SIZE and WRITE_SIZE cannot share a pass).
 # Summary: profiles/pmc_summary_r06.py (run in the build container: it prices the kernels' instruction mix from the assembly).
 export TMPDIR=/tmp; R=$GRAFT_REPO_ROOT; TAG=${1:-r06pmc}; N=${2:-8192}; O=$R/gpurun_out/$TAG; mkdir -p $O; cd $R
-W="python $R/tools/pmc_workload.py --reads $N --ea-reads $N --reps 2"
-V="python $R/tools/pmc_workload.py --var-tile 1 --reps 2"
-( cd /tmp && timeout 200 $W --timing-reps 5 > $O/units.json 2> $O/units.err ); echo "units rc=$?"        # the run WITHOUT counters: a warm-up step, five timed ones
-( cd /tmp && timeout 200 $V --timing-reps 5 > $O/units_variants.json 2> $O/units_variants.err ); echo "units variants rc=$?"
+W="python3 $R/tools/pmc_workload.py --reads $N --ea-reads $N --reps 2"
+V="python3 $R/tools/pmc_workload.py --var-tile 1 --reps 2"
+( cd /tmp && timeout 200 $W --timing-reps 5 > $O/units.json 2> $O/units.err )|| exit 1        # the run WITHOUT counters: a warm-up step, five timed ones
+( cd /tmp && timeout -k 10 150 $V --timing-reps 5 > $O/units_variants.json 2> $O/units_variants.err ) || exit 1
 pass() {   # name, workload, counters...
   local name=$1; local wl=$2; shift; shift
-  ( cd /tmp && timeout ${PASS_TIMEOUT:-200} rocprofv3 --kernel-trace --pmc "$@" --output-format csv -d $O/$name -o $name -- $wl > $O/$name.log 2>&1 ); echo "$name rc=$?" | tee -a $O/passes.log
+  ( cd /tmp && timeout -s KILL ${PASS_TIMEOUT:-150} rocprofv3 --kernel-trace --pmc "$@" --output-format csv -d $O/$name -o $name -- $wl > $O/$name.log 2>&1 ) || { echo "$name failed: no further pass"; exit 1; }
+  echo "$name ok" | tee -a $O/passes.log
 }
 pass sq1 "$W" SQ_INSTS_VALU SQ_INSTS_SALU SQ_ACTIVE_INST_VALU SQ_ACTIVE_INST_SCA SQ_BUSY_CYCLES SQ_WAVE_CYCLES SQ_WAIT_ANY SQ_WAIT_INST_ANY GRBM_GUI_ACTIVE
 pass fetch "$W" FETCH_SIZE

@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
-"""Summary of the round-6 counter passes (profiles/collect_r06_pmc.sh) -> profiles/r06_pmc.json.
+"""Summary of the counter passes of profiles/collect_r06_pmc.sh -> profiles/pmc_shipped.json (the shipped kernels; r06_pmc.json: an earlier state).
 
-    pmc_summary_r06.py gpurun_out/<tag>  [> profiles/r06_pmc.json]
+    pmc_summary_r06.py <folder of the passes>  [> profiles/pmc_shipped.json]
 
 Round 6 re-collects every family on the round's code (the recalibration kernel is new: np_recalibrate_half_kernel).  Round 5 added the families the round-4 review missed: the event detector of the from-raw / eventalign steps
 (np_ed_peaks_par_kernel<true> -- the fused t-statistics + peak walk --, np_ed_check_kernel, np_ed_events_kernel, np_mom_fill_kernel; unit =
@@ -98,7 +98,7 @@ try:
 except Exception as e:  # noqa: BLE001
     mix["error"] = repr(e)
 
-out = {"source": "rocprofv3 --kernel-trace --pmc over tools/pmc_workload.py (profiles/collect_r06_pmc.sh), gpurun tag %s" % root.rstrip("/").split("/")[-1],
+out = {"source": "rocprofv3 --kernel-trace --pmc over tools/pmc_workload.py (profiles/collect_r06_pmc.sh), pass folder %s" % root.rstrip("/").split("/")[-1],
        "units": units, "units_variants": units_var, "fetch_size_correction": FETCH_CORR, "write_size_correction": WRITE_CORR,
        "fast_class_cycles_per_instruction": FAST_CYCLES, "calibration": "profiles/r04_valu_calibration.json"}
 cm, ea, va = units.get("call_methylation", {}), units.get("eventalign", {}), units_var.get("variants", {})

@@ -1,12 +1,12 @@
 """Per-unit counter figures of the shipped kernels for the bench lines' `roofline.traffic` / `issue` fields, read from the committed
-summary of this round's counter passes (profiles/r06_pmc.json <- profiles/collect_r06_pmc.sh + profiles/pmc_summary_r06.py).  The passes
+summary of the counter passes over them (profiles/pmc_shipped.json <- profiles/collect_r06_pmc.sh + profiles/pmc_summary_r06.py).  The passes
 run at a launch size they finish at (8 192 reads); a bench line scales the PER-UNIT figures (bytes per band / call / segment) by the
 units its own launch processed, and says so in `source`."""
 import json
 import os
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-FILE = os.path.join("profiles", "r06_pmc.json")
+FILE = os.path.join("profiles", "pmc_shipped.json")
 
 
 def family(name):
