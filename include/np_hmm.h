@@ -211,7 +211,8 @@ int np_event_align_host(np_ctx* ctx, int n_jobs, const np_align_job* jobs,
  * C library that the reference runs on, so the PROCESS's own log / exp / logf form them.  np_mom_fill_dev, np_resolve_jobs_dev,
  * np_calibrate_resolve_dev and np_hmm_score_set_combine_dev enqueue a kernel that writes what they depend on into pinned host
  * memory, a host function (hipLaunchHostFunc) and a kernel that reads them back: in stream order, the caller does not wait.  These four
- * cannot be captured into a graph (NP_ERR_UNSUPPORTED). */
+ * cannot be captured into a graph (NP_ERR_UNSUPPORTED).  The pinned block is one per entry point and context: a caller that orders its
+ * streams itself ("stream_switch_wait" 0) orders two calls of the same entry point, as it does for the rest of the scratch. */
 
 /* Per-read record (device).  Filled by np_fill_read_host() on the host, then uploaded by the caller. */
 typedef struct np_read_dev {
