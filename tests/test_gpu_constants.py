@@ -140,3 +140,38 @@ def test_a_captured_call_is_refused(ctx, models):
     assert float(d_x[0]) == 1.0
     ctx._chk(ctx.L.np_mom_fill_dev(ctx.h, None, n, _p(d_rd), None, _p(d_ev), _p(d_ne), _p(d_rk), ctx.models["nucleotide"]), "np_mom_fill_dev")
     ctx.sync()
+
+
+def test_two_contexts_on_two_threads(models):
+    """Two contexts, a host thread each, their steps in flight side by side (ctypes releases the GIL): each forms its own constants."""
+    import threading
+    from nanopolish_amd.api import Context
+    from nanopolish_amd.pipeline import build_host_batch, tile_host_batch, CallMethylationBatch
+    hbs = [tile_host_batch(build_host_batch(models, ids, L=1000, raw=True), 30) for ids in ([20, 21, 22], [23, 24, 25, 26])]
+    ctxs, batches, want = [], [], []
+    for hb in hbs:
+        c = Context(0)
+        c.register_model(models["nucleotide"], "nucleotide"); c.register_model(models["cpg"], "cpg")
+        b = CallMethylationBatch(c, hb, "cuda:0", calibrate=True, from_raw=True)
+        b.step()
+        ctxs.append(c); batches.append(b); want.append((b.scores(), b.reads_aligned().tobytes(), b.reads_scored().tobytes()))
+    errors = []
+
+    def run(b):
+        try:
+            for _ in range(12):
+                b.step()
+            b.sync()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(b,)) for b in batches]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert errors == []
+    for b, w in zip(batches, want):
+        assert np.array_equal(b.scores(), w[0], equal_nan=True) and b.reads_aligned().tobytes() == w[1] and b.reads_scored().tobytes() == w[2]
+    for c in ctxs:
+        c.close()
